@@ -578,6 +578,298 @@ int64_t take_device_error() {
   return bits;
 }
 
+// ---- rotary positions and paged caches ----
+namespace {
+
+// Element strides of the leading dimensions; a dimension of one element has
+// none that matter and counts as `dense`.
+template <int kDims>
+void strides_of(const at::Tensor &t, int64_t (&s)[kDims], int64_t dense) {
+  for (int i = 0; i < kDims; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : dense;
+}
+
+void check_rows(const at::Tensor &t, const char *name, int64_t dims,
+                const char *layout) {
+  check_cuda(t, name);
+  check_16bit(t, name);
+  TORCH_CHECK(t.dim() == dims, name, " must be ", dims, "-D ", layout,
+              ", got ", t.dim(), "-D");
+  TORCH_CHECK(t.size(dims - 1) <= 1 || t.stride(dims - 1) == 1, name,
+              " must be contiguous along head_dim");
+}
+
+void check_freqs(const at::Tensor &freqs, const at::Tensor &like) {
+  check_cuda(freqs, "freqs");
+  check_contiguous(freqs, "freqs");
+  TORCH_CHECK(freqs.scalar_type() == at::kDouble,
+              "freqs must be float64 (got ", freqs.scalar_type(), ")");
+  TORCH_CHECK(freqs.dim() == 1 && freqs.size(0) > 0 &&
+                  2 * freqs.size(0) <= like.size(-1),
+              "freqs must be 1-D with one entry per rotated pair (at most "
+              "head_dim / 2), got ", freqs.sizes());
+  TORCH_CHECK(freqs.device() == like.device(),
+              "freqs must live on the device of the rows");
+}
+
+void check_int32(const at::Tensor &t, const char *name,
+                 const at::Tensor &like) {
+  check_cuda(t, name);
+  TORCH_CHECK(t.scalar_type() == at::kInt, name, " must be int32 (got ",
+              t.scalar_type(), ")");
+  TORCH_CHECK(t.device() == like.device(), name,
+              " must live on the device of the rows");
+}
+
+// The cache and the step of a paged call. `rows`: the packed tensor whose
+// first dimension counts the new tokens.
+void paged_call(const at::Tensor &rows, const at::Tensor &starts,
+                const at::Tensor &k_pages, const at::Tensor &v_pages,
+                const at::Tensor &page_table, const at::Tensor &seq_lens,
+                fa_paged_cache &c, fa_new_tokens &step) {
+  check_rows(k_pages, "k_pages", 4, "(pages, H_kv, rows, head_dim)");
+  check_rows(v_pages, "v_pages", 4, "(pages, H_kv, rows, head_dim)");
+  TORCH_CHECK(k_pages.sizes() == v_pages.sizes(),
+              "k_pages and v_pages must have identical shapes, got ",
+              k_pages.sizes(), " and ", v_pages.sizes());
+  TORCH_CHECK(k_pages.scalar_type() == rows.scalar_type() &&
+                  v_pages.scalar_type() == rows.scalar_type(),
+              "the new rows and the pages must have the same dtype, got ",
+              rows.scalar_type(), ", ", k_pages.scalar_type(), " and ",
+              v_pages.scalar_type());
+  const int64_t d = k_pages.size(3), page_rows = k_pages.size(2);
+  TORCH_CHECK(d == kHeadDim || d == 128, "k_pages must have head_dim == ",
+              kHeadDim, " (or 128), got ", d);
+  TORCH_CHECK(rows.size(-1) == d,
+              "the new rows and the pages must have the same head_dim, got ",
+              rows.size(-1), " and ", d);
+  TORCH_CHECK(k_pages.size(0) > 0 && k_pages.size(1) > 0,
+              "k_pages must hold at least one page and head, got ",
+              k_pages.sizes());
+  TORCH_CHECK(page_rows > 0 && page_rows % 8 == 0 &&
+                  (page_rows <= 128 || page_rows % 128 == 0),
+              "a page must have a multiple of 8 rows, and above 128 a "
+              "multiple of 128, got ", page_rows);
+  check_int32(starts, "starts", rows);
+  check_int32(seq_lens, "seq_lens", rows);
+  check_int32(page_table, "page_table", rows);
+  check_contiguous(starts, "starts");
+  check_contiguous(seq_lens, "seq_lens");
+  TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.size(0) > 0,
+              "seq_lens must be 1-D with one entry per sequence, got ",
+              seq_lens.sizes());
+  TORCH_CHECK(starts.dim() == 1 && starts.size(0) == seq_lens.size(0) + 1,
+              "starts must be 1-D of length B + 1 = ", seq_lens.size(0) + 1,
+              ", got ", starts.sizes());
+  TORCH_CHECK(page_table.dim() == 2 &&
+                  page_table.size(0) == seq_lens.size(0) &&
+                  page_table.size(1) > 0 &&
+                  (page_table.size(1) == 1 || page_table.stride(1) == 1),
+              "page_table must be (B, pages) with B=", seq_lens.size(0),
+              " and contiguous rows, got ", page_table.sizes());
+  TORCH_CHECK(k_pages.device() == rows.device() &&
+                  v_pages.device() == rows.device(),
+              "the new rows and the pages must live on the same device");
+  c = fa_paged_cache{};
+  int64_t s[3];
+  strides_of(k_pages, s, d);
+  c.k_pages = k_pages.data_ptr();
+  c.k_page_stride = s[0];
+  c.k_head_stride = s[1];
+  c.k_row_stride = s[2];
+  strides_of(v_pages, s, d);
+  c.v_pages = v_pages.data_ptr();
+  c.v_page_stride = s[0];
+  c.v_head_stride = s[1];
+  c.v_row_stride = s[2];
+  c.page_table = page_table.data_ptr<int32_t>();
+  c.table_stride = page_table.size(0) > 1 ? page_table.stride(0)
+                                          : page_table.size(1);
+  c.table_width = to_int(page_table.size(1), "page_table width");
+  c.num_pages = to_int(k_pages.size(0), "pages");
+  c.page_rows = to_int(page_rows, "page rows");
+  c.kv_heads = to_int(k_pages.size(1), "kv heads");
+  c.head_dim = static_cast<int32_t>(d);
+  step = fa_new_tokens{};
+  step.starts = starts.data_ptr<int32_t>();
+  step.seq_lens = seq_lens.data_ptr<int32_t>();
+  step.batch = to_int(seq_lens.size(0), "batch");
+  step.tokens = to_int(rows.size(0), "tokens");
+}
+
+}  // namespace
+
+// rope(q, k, positions, freqs, interleaved=False, inverse=False,
+// amplitude=1.0): rotary positions of q and (unless None) k, any strides in,
+// contiguous (B, H, N, head_dim) out. inverse=True is its gradient.
+py::tuple rope(const at::Tensor &q, const c10::optional<at::Tensor> &k,
+               const at::Tensor &positions, const at::Tensor &freqs,
+               bool interleaved, bool inverse, double amplitude) {
+  check_rows(q, "q", 4, "(B, H, N, head_dim)");
+  const int64_t d = q.size(3);
+  TORCH_CHECK(d > 0 && d <= 1024, "q must have head_dim in 1..1024, got ", d);
+  if (k) {
+    check_rows(*k, "k", 4, "(B, H_kv, N, head_dim)");
+    TORCH_CHECK(k->scalar_type() == q.scalar_type(),
+                "q and k must have the same dtype, got ", q.scalar_type(),
+                " and ", k->scalar_type());
+    TORCH_CHECK(k->size(0) == q.size(0) && k->size(2) == q.size(2) &&
+                    k->size(3) == d,
+                "q and k must agree on batch, length and head_dim, got q=",
+                q.sizes(), " k=", k->sizes());
+    TORCH_CHECK(k->device() == q.device(),
+                "q and k must live on the same device");
+  }
+  check_freqs(freqs, q);
+  check_int32(positions, "positions", q);
+  TORCH_CHECK(((positions.dim() == 1 && positions.size(0) == q.size(2)) ||
+               (positions.dim() == 2 && positions.size(0) == q.size(0) &&
+                positions.size(1) == q.size(2))) &&
+                  (positions.size(-1) <= 1 || positions.stride(-1) == 1),
+              "positions must be (N,) or (B, N) with contiguous rows, got ",
+              positions.sizes());
+  TORCH_CHECK(std::isfinite(amplitude), "amplitude must be finite");
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor qo = at::empty(q.sizes(), q.options());
+  at::Tensor ko = k ? at::empty(k->sizes(), k->options()) : at::Tensor();
+  if (q.numel() + (k ? k->numel() : 0) > 0) {
+    int64_t qs[3], ks[3] = {0, 0, 0};
+    strides_of(q, qs, d);
+    const bool has_k = k && k->numel() > 0;
+    if (has_k) strides_of(*k, ks, d);
+    TORCH_CHECK(q.numel() > 0, "q must not be empty where k is not, got ",
+                q.sizes());
+    check_status(
+        fa_rope(q.data_ptr(), qs, qo.data_ptr(),
+                has_k ? k->data_ptr() : nullptr, ks,
+                has_k ? ko.data_ptr() : nullptr, to_int(q.size(0), "batch"),
+                to_int(q.size(1), "heads"),
+                has_k ? to_int(k->size(1), "kv heads") : 0,
+                to_int(q.size(2), "sequence length"), static_cast<int>(d),
+                positions.data_ptr<int32_t>(),
+                positions.dim() == 2 && positions.size(0) > 1
+                    ? positions.stride(0)
+                    : 0,
+                freqs.data_ptr<double>(), static_cast<int>(2 * freqs.size(0)),
+                static_cast<float>(amplitude),
+                (interleaved ? FA_ROPE_INTERLEAVED : 0) |
+                    (inverse ? FA_ROPE_INVERSE : 0),
+                dtype_code(q), current_stream()),
+        "fa_rope");
+  }
+  return py::make_tuple(qo, k ? py::cast(ko) : py::object(py::none()));
+}
+
+// append_paged(k_new, v_new, starts, k_pages, v_pages, page_table, seq_lens,
+// q=None, freqs=None, positions=None, interleaved=False, amplitude=1.0):
+// stores the new rows in the pages (in place), rotated where freqs is given;
+// returns the rotated q (or None).
+py::object append_paged(const at::Tensor &k_new, const at::Tensor &v_new,
+                        const at::Tensor &starts, at::Tensor k_pages,
+                        at::Tensor v_pages, const at::Tensor &page_table,
+                        const at::Tensor &seq_lens,
+                        const c10::optional<at::Tensor> &q,
+                        const c10::optional<at::Tensor> &freqs,
+                        const c10::optional<at::Tensor> &positions,
+                        bool interleaved, double amplitude) {
+  check_rows(k_new, "k_new", 3, "(tokens, H_kv, head_dim)");
+  check_rows(v_new, "v_new", 3, "(tokens, H_kv, head_dim)");
+  TORCH_CHECK(k_new.sizes() == v_new.sizes() &&
+                  k_new.scalar_type() == v_new.scalar_type() &&
+                  k_new.device() == v_new.device(),
+              "k_new and v_new must agree on shape, dtype and device, got ",
+              k_new.sizes(), " and ", v_new.sizes());
+  fa_paged_cache c;
+  fa_new_tokens step;
+  paged_call(k_new, starts, k_pages, v_pages, page_table, seq_lens, c, step);
+  TORCH_CHECK(k_new.size(1) == c.kv_heads,
+              "k_new, v_new and the pages must agree on the head count, got ",
+              k_new.size(1), " and ", c.kv_heads);
+  if (q) {
+    check_rows(*q, "q", 3, "(tokens, H, head_dim)");
+    TORCH_CHECK(q->size(0) == k_new.size(0) && q->size(1) > 0 &&
+                    q->size(2) == c.head_dim &&
+                    q->scalar_type() == k_new.scalar_type() &&
+                    q->device() == k_new.device(),
+                "q must be (tokens, H, head_dim) of the new rows' dtype and "
+                "device, got ", q->sizes());
+    TORCH_CHECK(freqs.has_value(), "q is only rotated: freqs must be given");
+  }
+  if (freqs) check_freqs(*freqs, k_new);
+  if (positions) {
+    check_int32(*positions, "positions", k_new);
+    check_contiguous(*positions, "positions");
+    TORCH_CHECK(positions->dim() == 1 && positions->size(0) == k_new.size(0),
+                "positions must be 1-D with one entry per token, got ",
+                positions->sizes());
+  }
+  TORCH_CHECK(std::isfinite(amplitude), "amplitude must be finite");
+  const c10::cuda::CUDAGuard guard(k_new.device());
+  at::Tensor qo = q ? at::empty(q->sizes(), q->options()) : at::Tensor();
+  if (step.tokens > 0) {
+    int64_t qs[2] = {0, 0}, ks[2], vs[2];
+    strides_of(k_new, ks, c.head_dim);
+    strides_of(v_new, vs, c.head_dim);
+    if (q) strides_of(*q, qs, c.head_dim);
+    check_status(
+        fa_append_paged(q ? q->data_ptr() : nullptr, qs,
+                        q ? qo.data_ptr() : nullptr, k_new.data_ptr(), ks,
+                        v_new.data_ptr(), vs,
+                        q ? to_int(q->size(1), "heads") : 0, &c, &step,
+                        positions ? positions->data_ptr<int32_t>() : nullptr,
+                        freqs ? freqs->data_ptr<double>() : nullptr,
+                        freqs ? static_cast<int>(2 * freqs->size(0)) : 0,
+                        static_cast<float>(amplitude),
+                        interleaved ? FA_ROPE_INTERLEAVED : 0,
+                        dtype_code(k_new), current_stream()),
+        "fa_append_paged");
+  }
+  return q ? py::cast(qo) : py::object(py::none());
+}
+
+// attend_paged(q, starts, k_pages, v_pages, page_table, seq_lens, scale,
+// causal=True, return_lse=False): attention of the new tokens over the
+// paged cache, which already holds their rows.
+py::object attend_paged(const at::Tensor &q, const at::Tensor &starts,
+                        const at::Tensor &k_pages, const at::Tensor &v_pages,
+                        const at::Tensor &page_table,
+                        const at::Tensor &seq_lens, double scale, bool causal,
+                        bool return_lse) {
+  check_rows(q, "q", 3, "(tokens, H, head_dim)");
+  fa_paged_cache c;
+  fa_new_tokens step;
+  paged_call(q, starts, k_pages, v_pages, page_table, seq_lens, c, step);
+  TORCH_CHECK(q.size(1) > 0 && q.size(1) % c.kv_heads == 0 &&
+                  q.size(1) / c.kv_heads <= 128,
+              "q's head count must be a multiple (at most 128 times) of the "
+              "pages', got ", q.size(1), " and ", c.kv_heads);
+  TORCH_CHECK(std::isfinite(scale), "scale must be finite");
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor o = at::empty(q.sizes(), q.options());
+  at::Tensor lse;
+  if (return_lse)
+    lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+  if (step.tokens > 0) {
+    const size_t bytes = fa_attend_paged_workspace_bytes(c.head_dim, q.get_device());
+    TORCH_CHECK(bytes > 0, "fa_attend_paged_workspace_bytes failed");
+    const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+    DecodeScratch &ws = decode_scratch(q, bytes, static_cast<size_t>(sms));
+    int64_t qs[2];
+    strides_of(q, qs, c.head_dim);
+    check_status(
+        fa_attend_paged(
+            q.data_ptr(), qs, o.data_ptr(),
+            return_lse ? lse.data_ptr<float>() : nullptr,
+            to_int(q.size(1), "heads"), &c, &step, static_cast<float>(scale),
+            causal ? 1 : 0, dtype_code(q), ws.partials.data_ptr(),
+            static_cast<size_t>(ws.partials.numel()),
+            reinterpret_cast<uint32_t *>(ws.counters.data_ptr<int32_t>()),
+            static_cast<size_t>(ws.counters.numel()), current_stream()),
+        "fa_attend_paged");
+  }
+  if (return_lse) return py::make_tuple(o, lse);
+  return py::cast(o);
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "B200 (sm_100a) FlashAttention forward for head_dim=64";
   m.attr("head_dim") = kHeadDim;
@@ -626,6 +918,24 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("merge_partials", &merge_partials,
         "Merge (G, B, H, 68) decode partials into the fp16 output",
         py::arg("partials"));
+  m.def("rope", &rope,
+        "Rotary positions of q and k (inverse=True: the gradient)",
+        py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("freqs"),
+        py::arg("interleaved") = false, py::arg("inverse") = false,
+        py::arg("amplitude") = 1.0);
+  m.def("append_paged", &append_paged,
+        "Store new K/V rows in a paged cache, K (and q) rotated on the way",
+        py::arg("k_new"), py::arg("v_new"), py::arg("starts"),
+        py::arg("k_pages"), py::arg("v_pages"), py::arg("page_table"),
+        py::arg("seq_lens"), py::arg("q") = py::none(),
+        py::arg("freqs") = py::none(), py::arg("positions") = py::none(),
+        py::arg("interleaved") = false, py::arg("amplitude") = 1.0);
+  m.def("attend_paged", &attend_paged,
+        "Attention of a step's new tokens over a paged K/V cache",
+        py::arg("q"), py::arg("starts"), py::arg("k_pages"),
+        py::arg("v_pages"), py::arg("page_table"), py::arg("seq_lens"),
+        py::arg("scale"), py::arg("causal") = true,
+        py::arg("return_lse") = false);
   m.def("legacy_naive", &legacy_attention, "v1 single-head kernel (N, 64) fp32");
   m.def("legacy_tiled", &legacy_attention, "v1 single-head kernel (N, 64) fp32");
   m.def("legacy_fused", &legacy_attention, "v1 single-head kernel (N, 64) fp32");

@@ -10,3 +10,6 @@
 #include "legacy_sm100.cu"
 #include "noalloc.cu"
 #include "host_stage.cu"
+#include "rope_sm100.cu"
+#include "paged_attend_sm100.cu"
+#include "paged_capi.cu"

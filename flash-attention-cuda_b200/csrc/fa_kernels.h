@@ -123,6 +123,59 @@ int merge_threads();
 cudaError_t launch_merge_kernel(const float *partials, int G, __half *out,
                                 int B, int H, cudaStream_t stream);
 
+// ---- rotary positions and the paged append (rope_sm100.cu) ------------------
+struct RopeArgs {
+  const __half *q;  // null with H == 0: none
+  const __half *k;
+  const __half *v;  // append only
+  __half *q_out;
+  __half *k_out;  // append: the K pages
+  __half *v_out;  // append: the V pages
+  // element strides per batch entry, head and token
+  int64_t q_sb, q_sh, q_sn, qo_sb, qo_sh, qo_sn;
+  int64_t k_sb, k_sh, k_sn, ko_sb, ko_sh, ko_sn;
+  int64_t v_sh, v_sn;
+  int H, H_kv, N, D, rot;
+  int tokens;  // B * N, or the step's
+  const int32_t *positions;  // append: null for the cache row
+  int64_t position_stride;
+  const double *freqs;
+  float amplitude, sign;
+  int tokens_per_block, rows_per_block;  // set by the launch
+  // append
+  const int32_t *starts;
+  const int32_t *seq_lens;
+  const int32_t *page_table;
+  int64_t table_stride;
+  int64_t kp_sp, kp_sh, kp_sr, vp_sp, vp_sh, vp_sr;  // page, head, row
+  int batch, table_width, page_rows, num_pages;
+};
+// vector: every row is 16-byte aligned and rotates in whole 16-byte units.
+cudaError_t launch_rope_kernel(const RopeArgs &a, bool interleaved,
+                               bool append, bool vector, int dtype,
+                               cudaStream_t stream);
+
+// ---- attention over a paged cache (paged_attend_sm100.cu) -------------------
+struct PagedArgs {
+  const __half *q;
+  int64_t q_st, q_sh;  // element strides per token and head
+  __half *out;         // (tokens, H, D)
+  float *lse;          // (tokens, H) or null
+  const __half *k_pages;
+  const __half *v_pages;
+  int64_t kp_sp, kp_sh, kp_sr, vp_sp, vp_sh, vp_sr;
+  const int32_t *page_table;
+  int64_t table_stride;
+  const int32_t *starts;
+  const int32_t *seq_lens;
+  int batch, tokens, H, H_kv, D, table_width, page_rows, num_pages;
+  float scale_log2;
+  int causal;
+};
+size_t attend_paged_workspace_bytes(int head_dim, int sms);
+cudaError_t launch_attend_paged_kernel(const PagedArgs &a, int dtype,
+                                       cudaStream_t stream);
+
 // ---- single-head fp32 attention (legacy_sm100.cu) -------------------------
 cudaError_t launch_legacy_kernel(const float *q, const float *k, const float *v,
                                  float *o, int N, cudaStream_t stream);

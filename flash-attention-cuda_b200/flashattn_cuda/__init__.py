@@ -6,7 +6,9 @@ names with the same arguments for its head_dim-64 fp16 prefill and decode,
 backed by hand-written sm_100a kernels in libfa_b200.so. The same calls also
 take head_dim 128, bf16 tensors and K/V with fewer heads than Q; added are
 decode_append (cache append fused into decode), prefill_host (inputs in host
-memory, copies overlapped with the kernels), decode_partial / merge_partials
+memory, copies overlapped with the kernels), rotary positions (rope,
+rope_frequencies), caches in pages (append_paged, attend_paged: prompt chunks,
+drafted and single tokens in one call), decode_partial / merge_partials
 and flashattn_cuda.dist (multi-GPU sharding and the in-kernel NVLink decode
 exchange). There is no CPU or eager fallback: importing fails loudly if the
 compiled extension is missing.
@@ -18,6 +20,8 @@ import torch as _torch  # noqa: F401
 
 from ._C import (  # noqa: F401
     _decode_with_split,
+    append_paged,
+    attend_paged,
     choose_decode_split,
     decode,
     decode_append,
@@ -30,8 +34,10 @@ from ._C import (  # noqa: F401
     occupancy_report,
     prefill,
     prefill_host,
+    rope,
     take_device_error,
 )
+from .rotary import rope_frequencies  # noqa: F401
 
 __all__ = [
     "prefill",
@@ -46,6 +52,10 @@ __all__ = [
     "decode_append",
     "decode_partial",
     "merge_partials",
+    "rope",
+    "rope_frequencies",
+    "append_paged",
+    "attend_paged",
     "take_device_error",
 ]
 

@@ -39,6 +39,7 @@ extern "C" {
 /* Bits of the device-side error word (fa_take_device_error). */
 #define FA_ERR_TIMEOUT 1u   /* a pipeline wait exceeded its time limit   */
 #define FA_ERR_SMEM_ALIGN 2u /* dynamic shared memory was not 1 KiB aligned */
+#define FA_ERR_PAGE 4u /* a page table entry that was needed is not a page  */
 
 /* Element types of q/k/v/o and the caches for the _ex entry points (every
  * other entry point is fp16). */
@@ -440,6 +441,120 @@ int fa_set_wait_limit_ns(unsigned long long ns);
  */
 int fa_legacy_attention_f32(const float *q, const float *k, const float *v,
                             float *o, int N, void *stream);
+
+/*
+ * Rotary positions. Each of the rotary_dim / 2 pairs of a row's first
+ * rotary_dim elements is turned by the angle position * freqs[pair]
+ * (radians; freqs: rotary_dim / 2 doubles on the device) and multiplied by
+ * `amplitude`:
+ *   y0 = amplitude (x0 cos - x1 sin),  y1 = amplitude (x1 cos + x0 sin);
+ * the elements from rotary_dim on are copied. A pair is elements
+ * (i, i + rotary_dim / 2), or (2i, 2i + 1) with FA_ROPE_INTERLEAVED. With
+ * FA_ROPE_INVERSE the angle is negated, which makes the call the gradient of
+ * the forward call with the same arguments. Angles are formed in 64 bits, so
+ * far positions lose nothing; the rotation is fp32, rounded once.
+ *
+ * q (B, H, N, head_dim) and, unless NULL, k (B, H_kv, N, head_dim): element
+ * (b, h, n, d) lies at b * strides[0] + h * strides[1] + n * strides[2] + d
+ * (elements). q_out, k_out: contiguous (B, H, N, head_dim), the layout
+ * fa_prefill reads; they may be the inputs themselves where those are
+ * contiguous, and may not overlap them otherwise. positions: int32, that of
+ * (b, n) at b * position_stride + n (0: one row for every b). head_dim up to
+ * 1024, rotary_dim even, 2 <= rotary_dim <= head_dim. No reference
+ * counterpart (its callers rotate before prefill()).
+ */
+#define FA_ROPE_INTERLEAVED 1
+#define FA_ROPE_INVERSE 2
+int fa_rope(const void *q, const int64_t q_strides[3], void *q_out,
+            const void *k, const int64_t k_strides[3], void *k_out, int B,
+            int H, int H_kv, int N, int head_dim, const int32_t *positions,
+            int64_t position_stride, const double *freqs, int rotary_dim,
+            float amplitude, int flags, int dtype, void *stream);
+
+/*
+ * A K/V cache in pages. Row r of sequence b, head h is row r % page_rows of
+ * page page_table[b * table_stride + r / page_rows] of the pools; element
+ * (page, h, row, d) of a pool lies at page * page_stride + h * head_stride +
+ * row * row_stride + d (elements; strides are multiples of 8 and the pools
+ * 16-byte aligned, so both (pages, heads, rows, head_dim) and (pages, rows,
+ * heads, head_dim) pools serve). page_rows is a multiple of 8, and from 128
+ * rows on a multiple of 128. A sequence holds at most table_width *
+ * page_rows rows. head_dim is 64 or 128. Table entries past a sequence's
+ * rows are never read; one that is needed and is no page of the pool is
+ * neither read nor written through: it sets FA_ERR_PAGE in the device error
+ * word, and that sequence's results are undefined.
+ */
+typedef struct fa_paged_cache {
+  void *k_pages;
+  void *v_pages;
+  int64_t k_page_stride, k_head_stride, k_row_stride;
+  int64_t v_page_stride, v_head_stride, v_row_stride;
+  const int32_t *page_table;
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t num_pages;
+  int32_t page_rows;
+  int32_t kv_heads;
+  int32_t head_dim;
+} fa_paged_cache;
+
+/*
+ * The new tokens of a step, packed: sequence b's are rows starts[b] ..
+ * starts[b + 1] of the packed tensors (starts: batch + 1 int32 on the
+ * device, from 0, non-decreasing; none, one or many tokens a sequence), and
+ * seq_lens[b] (int32, device) is the sequence's rows INCLUDING them, so new
+ * token i of n stands at row seq_lens[b] - n + i. `tokens` is the packed
+ * tensors' row count; rows from starts[batch] on belong to no sequence and
+ * are left alone (a captured graph may be padded with them).
+ */
+typedef struct fa_new_tokens {
+  const int32_t *starts;
+  const int32_t *seq_lens;
+  int32_t batch;
+  int32_t tokens;
+} fa_new_tokens;
+
+/*
+ * Stores the new tokens' K and V rows in the cache, in one launch with their
+ * rotary positions: k_new is rotated on its way into the pages, and q (if
+ * given) into q_out. q (tokens, H, head_dim), k_new and v_new (tokens,
+ * kv_heads, head_dim): token t, head h at t * strides[0] + h * strides[1]
+ * (elements); q_out contiguous. freqs NULL: nothing is rotated (q must then
+ * be NULL too). positions: int32 per token, or NULL for the row the token is
+ * stored at. rotary_dim, amplitude, flags as fa_rope (FA_ROPE_INVERSE is
+ * refused). A token whose row is negative or past the table's capacity is
+ * not stored. No reference counterpart (see fa_decode_append).
+ */
+int fa_append_paged(const void *q, const int64_t q_strides[2], void *q_out,
+                    const void *k_new, const int64_t k_strides[2],
+                    const void *v_new, const int64_t v_strides[2], int H,
+                    const fa_paged_cache *cache, const fa_new_tokens *step,
+                    const int32_t *positions, const double *freqs,
+                    int rotary_dim, float amplitude, int flags, int dtype,
+                    void *stream);
+
+/*
+ * Attention of the new tokens over the paged cache: token i of sequence b
+ * attends rows [0, seq_lens[b]), or with causal != 0 rows [0, r] up to the
+ * row r it stands at. One token a sequence is the decode step, a few are
+ * drafted tokens being checked, many are a chunk of a prompt; one call takes
+ * any mix. q (tokens, H, head_dim) with strides as in fa_append_paged
+ * (multiples of 8), o contiguous (tokens, H, head_dim), H % kv_heads == 0
+ * and H / kv_heads <= 128. Scores, softmax and accumulators are fp32; the
+ * probabilities enter the second product in the tensors' 16-bit type. A
+ * token that sees no row gets zeros. lse, unless NULL: (tokens, H) fp32, the
+ * natural logarithm of each row's sum of exponentials (-inf where it sees
+ * no row). Rows of the pages past seq_lens[b] may hold anything.
+ * workspace: fa_attend_paged_workspace_bytes() bytes, 16-byte aligned, no
+ * initialisation; counters: as for fa_decode, at least as many as the device
+ * has SMs. No reference counterpart (its caches are contiguous).
+ */
+size_t fa_attend_paged_workspace_bytes(int head_dim, int device);
+int fa_attend_paged(const void *q, const int64_t q_strides[2], void *o,
+                    float *lse, int H, const fa_paged_cache *cache,
+                    const fa_new_tokens *step, float scale, int causal,
+                    int dtype, void *workspace, size_t workspace_bytes,
+                    uint32_t *counters, size_t counter_count, void *stream);
 
 /* Name of a status code. */
 const char *fa_status_string(int status);
