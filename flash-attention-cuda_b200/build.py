@@ -28,7 +28,8 @@ LIB_SOURCES = ["fa_all.cu", "capi.cu", "prefill_sm100.cu", "decode_sm100.cu",
                "prefill_d128_sm100.cu", "decode_d128_sm100.cu",
                "decode_gqa_sm100.cu",
                "noalloc.cu", "legacy_sm100.cu", "host_stage.cu",
-               "rope_sm100.cu", "paged_attend_sm100.cu", "paged_capi.cu",
+               "rope_sm100.cu", "paged_few_sm100.cu", "paged_many_sm100.cu",
+               "paged_attend_sm100.cu", "paged_sm100.cuh", "paged_capi.cu",
                "fa_sm100.cuh", "fa_kernels.h"]
 
 

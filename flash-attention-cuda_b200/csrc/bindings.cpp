@@ -852,7 +852,7 @@ py::object attend_paged(const at::Tensor &q, const at::Tensor &starts,
     const size_t bytes = fa_attend_paged_workspace_bytes(c.head_dim, q.get_device());
     TORCH_CHECK(bytes > 0, "fa_attend_paged_workspace_bytes failed");
     const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-    DecodeScratch &ws = decode_scratch(q, bytes, static_cast<size_t>(sms));
+    DecodeScratch &ws = decode_scratch(q, bytes, 2 * static_cast<size_t>(sms));
     int64_t qs[2];
     strides_of(q, qs, c.head_dim);
     check_status(

@@ -102,6 +102,18 @@ int ensure_device(int *device_out) {
         return st.status;
       }
     }
+    for (int i = 0; i < 2 * kPagedForms; ++i) {
+      const int form = i / 2, head_dim = i % 2 ? 128 : 64;
+      const void *fn = attend_paged_kernel_ptr(form, head_dim, dt);
+      if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               attend_paged_smem_bytes(form, head_dim)) !=
+              cudaSuccess ||
+          cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout,
+                               cudaSharedmemCarveoutMaxShared) != cudaSuccess) {
+        st.status = FA_ECUDA;
+        return st.status;
+      }
+    }
   }
   if (!g_encode) {
     void *fn = nullptr;

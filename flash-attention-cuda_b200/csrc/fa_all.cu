@@ -11,5 +11,7 @@
 #include "noalloc.cu"
 #include "host_stage.cu"
 #include "rope_sm100.cu"
+#include "paged_few_sm100.cu"
+#include "paged_many_sm100.cu"
 #include "paged_attend_sm100.cu"
 #include "paged_capi.cu"

@@ -171,10 +171,26 @@ struct PagedArgs {
   int batch, tokens, H, H_kv, D, table_width, page_rows, num_pages;
   float scale_log2;
   int causal;
+  // set by the launch: keys of a key tile, new tokens of an item, and the
+  // division of the work (paged_sm100.cuh)
+  int tile_keys, item_tokens, item_cost, min_piece;
+  float *partials;
+  uint32_t *counters;
 };
+// Form of the call: few query rows per sequence and K/V head
+// (paged_few_sm100.cu) or many (paged_many_sm100.cu).
+enum { kPagedFew = 0, kPagedMany = 1, kPagedForms = 2 };
+const void *attend_paged_kernel_ptr(int form, int head_dim, int dtype);
+int attend_paged_smem_bytes(int form, int head_dim);
 size_t attend_paged_workspace_bytes(int head_dim, int sms);
-cudaError_t launch_attend_paged_kernel(const PagedArgs &a, int dtype,
-                                       cudaStream_t stream);
+// Sets the fields above and launches; tm_q is used by kPagedMany.
+int attend_paged_form(const PagedArgs &a);
+void attend_paged_plan(PagedArgs &a, int form);
+cudaError_t launch_attend_paged_kernel(const PagedArgs &a, int form,
+                                       const CUtensorMap &tm_q,
+                                       const CUtensorMap &tm_k,
+                                       const CUtensorMap &tm_v, int dtype,
+                                       int sms, cudaStream_t stream);
 
 // ---- single-head fp32 attention (legacy_sm100.cu) -------------------------
 cudaError_t launch_legacy_kernel(const float *q, const float *k, const float *v,

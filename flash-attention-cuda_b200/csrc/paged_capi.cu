@@ -54,6 +54,29 @@ int check_cache(const fa_paged_cache *c) {
   return FA_OK;
 }
 
+// 4-D view of 16-bit elements (64 of the innermost a box), 128-byte swizzle;
+// what lies outside reads as zero. A dimension of one element takes any
+// stride.
+int make_map(CUtensorMap *map, const void *base, int dtype, const int (&sizes)[4],
+             const int64_t (&strides)[3], int box1, int box3) {
+  cuuint64_t dims[4], bytes[3];
+  for (int i = 0; i < 4; ++i) dims[i] = static_cast<cuuint64_t>(sizes[i]);
+  for (int i = 0; i < 3; ++i)
+    bytes[i] = 2 * static_cast<cuuint64_t>(sizes[i + 1] > 1 ? strides[i] : sizes[0]);
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box1), 1,
+                             static_cast<cuuint32_t>(box3)};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  return g_encode(map,
+                  dtype == FA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                  4, const_cast<void *>(base), dims, bytes, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? FA_OK
+             : FA_EINVAL;
+}
+
 int check_step(const fa_new_tokens *s) {
   if (!s || !s->starts || !s->seq_lens || s->batch <= 0 || s->tokens <= 0)
     return FA_EINVAL;
@@ -244,7 +267,7 @@ int fa_attend_paged(const void *q, const int64_t q_strides[2], void *o,
   if (H <= 0 || H % c.kv_heads != 0 || H / c.kv_heads > 128) return FA_EINVAL;
   if (static_cast<long long>(step->tokens) * H > INT_MAX) return FA_EINVAL;
   const int sizes[2] = {step->tokens, H};
-  if ((sizes[0] > 1 && q_strides[0] < 0) || (sizes[1] > 1 && q_strides[1] < 0))
+  if ((sizes[0] > 1 && q_strides[0] <= 0) || (sizes[1] > 1 && q_strides[1] <= 0))
     return FA_EINVAL;
   if (!aligned16(q) || !aligned16(o) || !strides_vector(q_strides, sizes, 2) ||
       !aligned16(workspace) || !aligned4(lse) || !aligned4(counters))
@@ -254,7 +277,7 @@ int fa_attend_paged(const void *q, const int64_t q_strides[2], void *o,
   if (rc != FA_OK) return rc;
   const int sms = g_devices[dev].sms;
   if (workspace_bytes < attend_paged_workspace_bytes(c.head_dim, sms) ||
-      counter_count < static_cast<size_t>(sms))
+      counter_count < 2 * static_cast<size_t>(sms))
     return FA_ENOSPACE;
 
   PagedArgs a{};
@@ -285,7 +308,28 @@ int fa_attend_paged(const void *q, const int64_t q_strides[2], void *o,
   a.D = c.head_dim;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.causal = causal != 0;
-  return launch_attend_paged_kernel(a, dtype,
+  a.partials = static_cast<float *>(workspace);
+  a.counters = counters;
+  const int form = attend_paged_form(a);
+  attend_paged_plan(a, form);
+  const int group = H / c.kv_heads;
+  const int box = c.page_rows < 128 ? c.page_rows : 128;
+  const int kv_sizes[4] = {c.head_dim, c.page_rows, c.kv_heads, c.num_pages};
+  const int64_t k_str[3] = {c.k_row_stride, c.k_head_stride, c.k_page_stride};
+  const int64_t v_str[3] = {c.v_row_stride, c.v_head_stride, c.v_page_stride};
+  CUtensorMap tq{}, tk, tv;
+  if (make_map(&tk, c.k_pages, dtype, kv_sizes, k_str, box, 1) != FA_OK ||
+      make_map(&tv, c.v_pages, dtype, kv_sizes, v_str, box, 1) != FA_OK)
+    return FA_EINVAL;
+  if (form == kPagedMany) {
+    // (dims, heads of a group, groups, tokens): a box is a tile's rows in
+    // the order (token, head)
+    const int q_sizes[4] = {c.head_dim, group, c.kv_heads, step->tokens};
+    const int64_t q_str[3] = {q_strides[1], q_strides[1] * group, q_strides[0]};
+    if (make_map(&tq, q, dtype, q_sizes, q_str, group, a.item_tokens / 2) != FA_OK)
+      return FA_EINVAL;
+  }
+  return launch_attend_paged_kernel(a, form, tq, tk, tv, dtype, sms,
                                     static_cast<cudaStream_t>(stream)) ==
                  cudaSuccess
              ? FA_OK

@@ -1,0 +1,457 @@
+// Attention of few new tokens per sequence over a paged K/V cache: the
+// decode step and drafted tokens (fa_attend_paged where a K/V head has at
+// most a few query rows per sequence).
+//
+//   o_i = sum_j exp(scale q_i k_j - m_i) v_j / l_i,  j over the rows that
+//   token i sees, m_i and l_i the running maximum and sum.
+//
+// Bound: HBM, each K/V row is read once for the 16 query rows (new token,
+// head of the group) that share it. One CTA per SM: a producer warp streams
+// key tiles (K and V, up to 128 rows, one TMA box per page and 64 dims) into
+// a ring that holds 192 KiB, eight consumer warps take 16 keys of every tile
+// each, with their own running softmax and accumulators (warp-level MMAs on
+// 16-row blocks: at so few rows the tensor work is a small part of the
+// tile's HBM time, and a 128-row tcgen05 tile would be mostly padding). Their
+// states are joined through shared memory at the end of a part. P enters the
+// second product rounded to the tensors' 16-bit type, as the MMA takes it.
+
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "fa_kernels.h"
+#include "fa_sm100.cuh"
+#include "paged_sm100.cuh"
+
+namespace fa {
+namespace paged {
+namespace few {
+
+constexpr int kRows = 16;  // query rows of an item
+constexpr int kWarps = 8;  // consumers
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr float kNegBig = -1e30f;  // the maximum of no scores yet
+
+template <int D>
+struct Cfg {
+  static constexpr uint32_t kHalf = kTileRows * 128;   // 64 dims of a tile
+  static constexpr uint32_t kTile = D / 64 * kHalf;    // K or V
+  static constexpr uint32_t kStage = 2 * kTile;
+  static constexpr int kStages = 6 * 64 / D;           // 192 KiB
+  static constexpr int kChunk = 32;  // dims joined at a time
+  static constexpr uint32_t kRedOff = kStages * kStage;
+  static constexpr uint32_t kRedBytes = kWarps * kRows * kChunk * 4;
+  static constexpr uint32_t kStatOff = kRedOff + kRedBytes;  // (m, l) per warp, row
+  static constexpr uint32_t kStatBytes = kWarps * kRows * 8;
+  static constexpr uint32_t kBarOff = kStatOff + kStatBytes;
+  // full[stage], empty[stage], consumers
+  static constexpr uint32_t kMiscOff = kBarOff + (2 * kStages + 1) * 8;
+  static constexpr uint32_t kSmemBytes = kMiscOff + sizeof(PlanSmem) + 16;
+  static_assert(kSmemBytes + 1024 <= 228 * 1024, "above the SM's shared memory");
+  static constexpr int kSlotFloats = kRows * (D + 2);  // a partial: O, m, l
+};
+
+// A bounded barrier of the consumer warps.
+struct Sync {
+  uint64_t *bar;
+  uint32_t phase = 0;
+  __device__ __forceinline__ bool operator()() {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+    const bool ok = mbar_wait(bar, phase);
+    phase ^= 1;
+    return ok;
+  }
+};
+
+// Row r of an item: new token r / group of it, head r % group of the group.
+struct Row {
+  int token, head;  // packed token, query head; token -1: no row
+  int seen;
+};
+__device__ __forceinline__ Row row_of(const PagedArgs &a, const Part &it, int r) {
+  const int group = a.H / a.H_kv;
+  const int tok = r / group;
+  Row w;
+  const bool has = tok < a.item_tokens && it.token + tok < it.seq.n;
+  w.token = has ? it.seq.lo + it.token + tok : -1;
+  w.head = it.h * group + r - tok * group;
+  w.seen = has ? rows_seen(a, it.seq, it.token + tok) : 0;
+  return w;
+}
+
+template <int D>
+__device__ __forceinline__ void store_result(const PagedArgs &a, const Row &w,
+                                             int dim, float2 x, float m,
+                                             float l, int dtype) {
+  const size_t row = static_cast<size_t>(w.token) * a.H + w.head;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const uint32_t v = dtype == FA_DTYPE_BF16 ? BF16::pack2(x.x * inv, x.y * inv)
+                                            : F16::pack2(x.x * inv, x.y * inv);
+  *reinterpret_cast<uint32_t *>(a.out + row * D + dim) = v;
+  if (dim == 0 && a.lse)
+    a.lse[row] = l == 0.f ? -INFINITY : 0.69314718055994531f * (m + log2f(l));
+}
+
+// Joins the partials of a split item (by the CTA that finished last).
+template <int D>
+__device__ __forceinline__ bool join(const PagedArgs &a, const Division &d,
+                                     const Part &it, int n_rows, float *red,
+                                     Sync &sync, int dtype) {
+  using C = Cfg<D>;
+  const int tid = threadIdx.x;  // 256 consumers
+  const int c0 = d.owner(it.at), c1 = d.owner(it.at + it.cost - 1);
+  // groups of threads share a row's dims; the groups take every n-th CTA
+  const int units = n_rows * (D / 4);
+  const int groups = max(1, 32 * kWarps / units);
+  for (int u0 = 0; u0 < units; u0 += 32 * kWarps) {
+    const int g = groups > 1 ? tid / units : 0;
+    const int u = groups > 1 ? tid % units : u0 + tid;
+    const bool on = g < groups && u < units;
+    const int row = u / (D / 4), d4 = u % (D / 4);
+    float m = kNegBig, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (on) {
+#pragma unroll 4
+      for (int c = c0 + g; c <= c1; c += groups) {
+        int t0, t1;
+        tiles_of_cta(a, d, it, c, t0, t1);
+        if (t0 >= t1) continue;
+        const float *p = a.partials +
+                         (2 * static_cast<size_t>(c) + slot_of(t0)) * C::kSlotFloats;
+        const float mc = __ldcg(p + kRows * D + row);
+        const float lc = __ldcg(p + kRows * D + kRows + row);
+        const float4 oc = __ldcg(reinterpret_cast<const float4 *>(p + row * D) + d4);
+        if (lc == 0.f) continue;  // saw nothing
+        const float mn = fmaxf(m, mc);
+        const float s0 = fast_exp2(m - mn), s1 = fast_exp2(mc - mn);
+        m = mn;
+        l = l * s0 + lc * s1;
+        acc.x = acc.x * s0 + oc.x * s1;
+        acc.y = acc.y * s0 + oc.y * s1;
+        acc.z = acc.z * s0 + oc.z * s1;
+        acc.w = acc.w * s0 + oc.w * s1;
+      }
+    }
+    if (groups > 1) {
+      float *mine = red + tid * 6;
+      mine[0] = m;
+      mine[1] = l;
+      mine[2] = acc.x;
+      mine[3] = acc.y;
+      mine[4] = acc.z;
+      mine[5] = acc.w;
+      if (!sync()) return false;
+      if (on && g == 0) {
+        for (int o = 1; o < groups; ++o) {
+          const float *p = red + (tid + o * units) * 6;
+          if (p[1] == 0.f) continue;
+          const float mn = fmaxf(m, p[0]);
+          const float s0 = fast_exp2(m - mn), s1 = fast_exp2(p[0] - mn);
+          m = mn;
+          l = l * s0 + p[1] * s1;
+          acc.x = acc.x * s0 + p[2] * s1;
+          acc.y = acc.y * s0 + p[3] * s1;
+          acc.z = acc.z * s0 + p[4] * s1;
+          acc.w = acc.w * s0 + p[5] * s1;
+        }
+      }
+    }
+    if (on && g == 0) {
+      const Row w = row_of(a, it, row);
+      store_result<D>(a, w, 4 * d4, make_float2(acc.x, acc.y), m, l, dtype);
+      store_result<D>(a, w, 4 * d4 + 2, make_float2(acc.z, acc.w), m, l, dtype);
+    }
+  }
+  return sync();  // red is free again
+}
+
+template <int D, typename Dt>
+__device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
+                        uint8_t *smem, uint64_t *full, uint64_t *empty,
+                        Sync sync) {
+  using C = Cfg<D>;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int quad = lane >> 2;  // MMA rows quad and quad + 8
+  const int qid = lane & 3;    // MMA column pair
+  const int key0 = warp * 16;  // this warp's keys within a tile
+  float *red = reinterpret_cast<float *>(smem + C::kRedOff);
+  float2 *stat = reinterpret_cast<float2 *>(smem + C::kStatOff);
+  int *last = reinterpret_cast<int *>(smem + C::kMiscOff + sizeof(PlanSmem));
+
+  int pos = 0;  // ring position
+  Part it;
+  while (walk.next(a, it)) {
+    const Row w0 = row_of(a, it, quad), w1 = row_of(a, it, quad + 8);
+    uint32_t qa[D / 16][4];  // Q as the A operand, dims 16kk..16kk+16
+    {
+      const uint32_t *q0 = w0.token >= 0 ? reinterpret_cast<const uint32_t *>(
+          a.q + w0.token * a.q_st + w0.head * a.q_sh) : nullptr;
+      const uint32_t *q1 = w1.token >= 0 ? reinterpret_cast<const uint32_t *>(
+          a.q + w1.token * a.q_st + w1.head * a.q_sh) : nullptr;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        qa[kk][0] = q0 ? q0[8 * kk + qid] : 0u;
+        qa[kk][1] = q1 ? q1[8 * kk + qid] : 0u;
+        qa[kk][2] = q0 ? q0[8 * kk + 4 + qid] : 0u;
+        qa[kk][3] = q1 ? q1[8 * kk + 4 + qid] : 0u;
+      }
+    }
+    float o[D / 8][4];  // dims 8dt + 2qid (+1), rows quad / quad + 8
+#pragma unroll
+    for (int dt = 0; dt < D / 8; ++dt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[dt][e] = 0.f;
+    float m0 = kNegBig, m1 = kNegBig, l0 = 0.f, l1 = 0.f;
+
+    for (int i = it.t0; i < it.t1; ++i, ++pos) {
+      const int slot = pos % C::kStages;
+      if (!mbar_wait(&full[slot], (pos / C::kStages) & 1)) return;
+      const int base = i * a.tile_keys;
+      // rows of this warp that the tile holds
+      const int here = min(it.keys - base, a.tile_keys) - key0;
+      if (here > 0) {  // warp-uniform
+        const uint32_t kb = smem_u32(smem + slot * C::kStage);
+        const uint32_t vb = kb + C::kTile;
+        float sc[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[j][e] = 0.f;
+          const int row = key0 + 8 * j + (lane & 7);
+#pragma unroll
+          for (int pp = 0; pp < D / 32; ++pp) {
+            const int chunk = 4 * (pp & 1) + (lane >> 3);
+            uint32_t kf[4];
+            ldsm_x4(kb + (pp >> 1) * C::kHalf + row * 128 +
+                        ((chunk ^ (row & 7)) << 4), kf);
+            Dt::mma16816(sc[j], qa[2 * pp], kf[0], kf[1]);
+            Dt::mma16816(sc[j], qa[2 * pp + 1], kf[2], kf[3]);
+          }
+        }
+        // rows past the sequence, or past what the token sees, hold anything
+        const int s0 = min(w0.seen - base - key0, here);
+        const int s1 = min(w1.seen - base - key0, here);
+        float x[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[j][e] = 8 * j + 2 * qid + (e & 1) < (e < 2 ? s0 : s1)
+                          ? sc[j][e] * a.scale_log2 : -INFINITY;
+        float mx0 = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
+        float mx1 = fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]));
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+        const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+        const float corr0 = fast_exp2(m0 - n0), corr1 = fast_exp2(m1 - n1);
+        m0 = n0;
+        m1 = n1;
+        float p[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          p[j][0] = fast_exp2(x[j][0] - n0);
+          p[j][1] = fast_exp2(x[j][1] - n0);
+          p[j][2] = fast_exp2(x[j][2] - n1);
+          p[j][3] = fast_exp2(x[j][3] - n1);
+        }
+        l0 = fmaf(l0, corr0, (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]));
+        l1 = fmaf(l1, corr1, (p[0][2] + p[0][3]) + (p[1][2] + p[1][3]));
+#pragma unroll
+        for (int dt = 0; dt < D / 8; ++dt) {
+          o[dt][0] *= corr0;
+          o[dt][1] *= corr0;
+          o[dt][2] *= corr1;
+          o[dt][3] *= corr1;
+        }
+        const uint32_t pa[4] = {Dt::pack2(p[0][0], p[0][1]),
+                                Dt::pack2(p[0][2], p[0][3]),
+                                Dt::pack2(p[1][0], p[1][1]),
+                                Dt::pack2(p[1][2], p[1][3])};
+        // V rows past the sequence may be NaN: zero times them is not zero
+        uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+        if (here < 16) {
+          keep0 = (2 * qid < here ? 0xffffu : 0u) |
+                  (2 * qid + 1 < here ? 0xffff0000u : 0u);
+          keep1 = (8 + 2 * qid < here ? 0xffffu : 0u) |
+                  (9 + 2 * qid < here ? 0xffff0000u : 0u);
+        }
+        const int vrow = key0 + 8 * ((lane >> 3) & 1) + (lane & 7);
+#pragma unroll
+        for (int dp = 0; dp < D / 16; ++dp) {
+          const int chunk = 2 * dp + (lane >> 4);
+          uint32_t vf[4];
+          ldsm_x4_trans(vb + (chunk >> 3) * C::kHalf + vrow * 128 +
+                            (((chunk & 7) ^ (vrow & 7)) << 4), vf);
+          Dt::mma16816(o[2 * dp], pa, vf[0] & keep0, vf[1] & keep1);
+          Dt::mma16816(o[2 * dp + 1], pa, vf[2] & keep0, vf[3] & keep1);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[slot]);
+    }
+
+    // ---- the warps' states, joined
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    if (qid == 0) {
+      stat[warp * kRows + quad] = make_float2(m0, l0);
+      stat[warp * kRows + quad + 8] = make_float2(m1, l1);
+    }
+    if (!sync()) return;
+    float M0 = kNegBig, M1 = kNegBig;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      M0 = fmaxf(M0, stat[i * kRows + quad].x);
+      M1 = fmaxf(M1, stat[i * kRows + quad + 8].x);
+    }
+    const float f0 = fast_exp2(m0 - M0), f1 = fast_exp2(m1 - M1);
+    const int group = a.H / a.H_kv;
+    const int n_rows = min(a.item_tokens, it.seq.n - it.token) * group;
+    float *slot = a.partials + (2 * static_cast<size_t>(blockIdx.x) +
+                                slot_of(it.t0)) * C::kSlotFloats;
+    const bool whole = it.whole();
+#pragma unroll
+    for (int ch = 0; ch < D / C::kChunk; ++ch) {
+      constexpr int kDt = C::kChunk / 8;
+#pragma unroll
+      for (int e = 0; e < kDt; ++e) {
+        const int dt = ch * kDt + e;
+        float *r = red + (warp * kRows + quad) * C::kChunk + 8 * e + 2 * qid;
+        if (quad < n_rows)
+          *reinterpret_cast<float2 *>(r) = make_float2(o[dt][0] * f0, o[dt][1] * f0);
+        if (quad + 8 < n_rows)
+          *reinterpret_cast<float2 *>(r + 8 * C::kChunk) =
+              make_float2(o[dt][2] * f1, o[dt][3] * f1);
+      }
+      if (!sync()) return;
+      // thread: row tid / 16, dims 2 (tid % 16) (+1) of the chunk
+      const int r = threadIdx.x >> 4, c = 2 * (threadIdx.x & 15);
+      if (r < n_rows) {
+        float2 sum = make_float2(0.f, 0.f);
+        float M = kNegBig, L = 0.f;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+          const float2 v = *reinterpret_cast<const float2 *>(
+              red + (i * kRows + r) * C::kChunk + c);
+          sum.x += v.x;
+          sum.y += v.y;
+          M = fmaxf(M, stat[i * kRows + r].x);
+        }
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i)
+          L += stat[i * kRows + r].y * fast_exp2(stat[i * kRows + r].x - M);
+        const int dim = ch * C::kChunk + c;
+        if (whole) {
+          store_result<D>(a, row_of(a, it, r), dim, sum, M, L, Dt::kDtype);
+        } else {
+          *reinterpret_cast<float2 *>(slot + r * D + dim) = sum;
+          if (dim == 0) {
+            slot[kRows * D + r] = M;
+            slot[kRows * D + kRows + r] = L;
+          }
+        }
+      }
+      if (!whole && ch == D / C::kChunk - 1) __threadfence();
+      if (!sync()) return;
+    }
+    if (!whole) {
+      // the part that completes the item's tiles joins them
+      uint32_t *counter = a.counters + d.owner(it.at);
+      if (threadIdx.x == 0) {
+        const uint32_t had = atomicAdd(counter, it.t1 - it.t0);
+        *last = had + (it.t1 - it.t0) == static_cast<uint32_t>(it.tiles);
+        if (*last) *counter = 0;
+        __threadfence();
+      }
+      if (!sync()) return;
+      if (*last && !join<D>(a, d, it, n_rows, red, sync, Dt::kDtype)) return;
+      if (!sync()) return;
+    }
+  }
+}
+
+template <int D, typename Dt>
+__global__ void __launch_bounds__(kThreads, 1)
+    attend_few_kernel(const PagedArgs a, const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v) {
+  using C = Cfg<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::kBarOff);
+  uint64_t *empty = full + C::kStages;
+  uint64_t *consumers = empty + C::kStages;
+  PlanSmem *ps = reinterpret_cast<PlanSmem *>(smem + C::kMiscOff);
+  int *failed = reinterpret_cast<int *>(smem + C::kMiscOff + sizeof(PlanSmem)) + 1;
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) record_error(FA_ERR_SMEM_ALIGN);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kWarps);
+    }
+    mbar_init(consumers, kWarps);
+    fence_barrier_init();
+    prefetch_tensormap(&tm_k);
+    prefetch_tensormap(&tm_v);
+    *failed = device_failed();
+  }
+  Division d;
+  Walk walk;
+  if (!plan<kThreads>(a, *ps, d, walk)) return;  // synchronises the CTA
+  if (*failed) return;
+
+  if (warp < kWarps) {
+    consume<D, Dt>(a, d, walk, smem, full, empty, Sync{consumers});
+    return;
+  }
+  // ---- producer: lane j loads page j of the tile
+  const int box = min(a.page_rows, kTileRows);
+  int pos = 0;
+  bool ok = true;
+  Part it;
+  while (ok && walk.next(a, it)) {
+    int page = it.t0 < it.t1 ? tile_page(a, it.b, it.keys, it.t0, lane) : -1;
+    for (int i = it.t0; i < it.t1; ++i, ++pos) {
+      const int next = i + 1 < it.t1 ? tile_page(a, it.b, it.keys, i + 1, lane) : -1;
+      const int slot = pos % C::kStages, use = pos / C::kStages;
+      if (use > 0 && !mbar_wait(&empty[slot], (use - 1) & 1)) {
+        ok = false;
+        break;
+      }
+      const uint32_t pages = __ballot_sync(0xffffffffu, page >= 0);
+      if (lane == 0)
+        mbar_arrive_expect_tx(&full[slot], __popc(pages) * box * 128 * (D / 64) * 2);
+      __syncwarp();
+      if (page >= 0) {
+        const int row = a.page_rows < kTileRows ? 0 : i * a.tile_keys % a.page_rows;
+        uint8_t *to = smem + slot * C::kStage + lane * box * 128;
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+          tma_load_4d(to + h * C::kHalf, &tm_k, &full[slot], 64 * h, row, it.h, page);
+          tma_load_4d(to + C::kTile + h * C::kHalf, &tm_v, &full[slot], 64 * h, row,
+                      it.h, page);
+        }
+      }
+      page = next;
+    }
+  }
+  // No copy may still be landing when the CTA exits: the consumers wait for
+  // all of them unless a wait ran out.
+  for (int p = pos > C::kStages ? pos - C::kStages : 0; p < pos; ++p)
+    mbar_wait(&full[p % C::kStages], (p / C::kStages) & 1);
+}
+
+}  // namespace few
+}  // namespace paged
+}  // namespace fa

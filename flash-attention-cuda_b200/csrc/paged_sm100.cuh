@@ -1,0 +1,266 @@
+// What the paged attention kernels share: the key tiles of a paged cache and
+// how a step's work is divided over the grid.
+//
+// Work: an item is a (sequence, K/V head, block of new tokens); its query
+// rows are (token, head of the group), so a K/V row is read once for all of
+// them. Items vary from one row to two full tiles and from no key to the
+// whole cache, and only the device knows the lengths. So every CTA adds up
+// the step's cost (keys per item plus a constant for starting and finishing
+// one), takes the piece [u0, u1) of it that its index gives, and walks the
+// items of that piece in order. A piece may begin and end inside an item's
+// keys; the parts of such an item are joined by whichever of its CTAs
+// finishes last (the sum of their tile counts tells), in the order of the
+// CTAs, so results do not depend on timing. Nothing waits on another CTA.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "fa_kernels.h"
+#include "fa_sm100.cuh"
+
+namespace fa {
+namespace paged {
+
+// 4-D tiled TMA load; coordinates are innermost first.
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map,
+                                            uint64_t *bar, int c0, int c1,
+                                            int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_"
+      "tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0),
+      "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+constexpr int kTileRows = 128;  // key rows a tile has room for
+
+// Keys of a tile: the whole pages that fit, or 128 rows of a larger page.
+__host__ __device__ inline int tile_keys(int page_rows) {
+  return page_rows < kTileRows ? kTileRows / page_rows * page_rows : kTileRows;
+}
+
+// One sequence of the step.
+struct Seq {
+  int lo;          // first packed token
+  int n;           // new tokens
+  long long len;   // cache rows with them (as given)
+};
+
+__host__ __device__ __forceinline__ Seq read_seq(const PagedArgs &a, int b) {
+  Seq s;
+  s.lo = min(max(a.starts[b], 0), a.tokens);
+  s.n = min(max(a.starts[b + 1], s.lo), a.tokens) - s.lo;
+  s.len = a.seq_lens[b];
+  return s;
+}
+
+// Cost of the first p items of one K/V head of a sequence, each of them full
+// (a.item_tokens tokens): a.item_cost and the keys up to its last token.
+__host__ __device__ __forceinline__ long long cost_before(const PagedArgs &a,
+                                                 const Seq &s, long long p) {
+  if (!a.causal) return p * (a.item_cost + max(s.len, 0ll));
+  const long long t = a.item_tokens, c = s.len - s.n;
+  const long long z = c < 0 ? min(p, -c / t) : 0;  // items that end before row 0
+  return p * a.item_cost + (p - z) * c + t * (p * (p + 1) - z * (z + 1)) / 2;
+}
+__host__ __device__ __forceinline__ int items_of(const PagedArgs &a, const Seq &s) {
+  return (s.n + a.item_tokens - 1) / a.item_tokens;
+}
+__host__ __device__ __forceinline__ long long cost_of(const PagedArgs &a, const Seq &s) {
+  return s.n == 0 ? 0
+                  : cost_before(a, s, items_of(a, s) - 1) + a.item_cost +
+                        max(s.len, 0ll);
+}
+
+// The part of an item that a CTA has.
+struct Part {
+  int b, h;        // sequence, K/V head
+  int token;       // first new token of the item within the sequence
+  Seq seq;
+  int keys;        // rows of the sequence in the cache (0..capacity)
+  int tiles;       // key tiles of the item
+  int t0, t1;      // those of this part
+  long long at, cost;  // the item's place in the step's cost
+  __host__ __device__ bool whole() const { return t0 == 0 && t1 == tiles; }
+};
+
+// The step's division, the same in every CTA.
+struct Division {
+  long long total;
+  int ctas;  // CTAs with work
+  __host__ __device__ long long piece(long long c) const { return c * total / ctas; }
+  // the CTA whose piece holds position u
+  __host__ __device__ int owner(long long u) const {
+    return static_cast<int>(((u + 1) * ctas - 1) / total);
+  }
+};
+
+// Rows that a token sees of its sequence.
+__host__ __device__ __forceinline__ int rows_seen(const PagedArgs &a, const Seq &s,
+                                         long long token) {
+  const long long cap = static_cast<long long>(a.table_width) * a.page_rows;
+  const long long r = a.causal ? s.len - s.n + token + 1 : s.len;
+  return static_cast<int>(max(0ll, min(min(r, s.len), cap)));
+}
+
+// The first tile that a position inside an item leaves to its right.
+__host__ __device__ __forceinline__ int tile_at(const PagedArgs &a, int tiles,
+                                       long long x) {
+  const long long k = x - a.item_cost;
+  return k <= 0 ? 0
+                : static_cast<int>(
+                      min(static_cast<long long>(tiles), (k + a.tile_keys - 1) / a.tile_keys));
+}
+
+// Walks the parts of one CTA.
+struct Walk {
+  long long u0, u1, at;
+  int b, h, p;
+  Seq s;
+
+  __host__ __device__ bool next(const PagedArgs &a, Part &out) {
+    while (at < u1) {
+      if (p >= items_of(a, s)) {  // the next head, or sequence with new tokens
+        p = 0;
+        if (++h == a.H_kv) {
+          h = 0;
+          do {
+            if (++b >= a.batch) return false;
+            s = read_seq(a, b);
+          } while (s.n == 0);
+        }
+      }
+      const int first = p * a.item_tokens;
+      const int last = min(first + a.item_tokens, s.n) - 1;
+      const long long c = s.len - s.n;
+      out.b = b;
+      out.h = h;
+      out.token = first;
+      out.seq = s;
+      out.at = at;
+      out.cost = a.item_cost + max(0ll, a.causal ? c + last + 1 : s.len);
+      out.keys = rows_seen(a, s, s.n - 1);
+      out.tiles = (rows_seen(a, s, last) + a.tile_keys - 1) / a.tile_keys;
+      out.t0 = at >= u0 ? 0 : tile_at(a, out.tiles, u0 - at);
+      out.t1 = at + out.cost <= u1 ? out.tiles : tile_at(a, out.tiles, u1 - at);
+      const bool mine = out.tiles == 0 ? at >= u0 : out.t0 < out.t1;
+      at += out.cost;
+      ++p;
+      if (mine) return true;
+    }
+    return false;
+  }
+};
+
+// The walk of the piece [u0, u1), which begins in sequence b, whose items
+// begin at position `at` of the step's cost.
+__host__ __device__ __forceinline__ void start(const PagedArgs &a, Walk &w,
+                                               int b, long long at) {
+  w.b = b;
+  w.s = read_seq(a, b);
+  const long long head = cost_of(a, w.s);
+  w.h = static_cast<int>((w.u0 - at) / head);
+  const long long x = w.u0 - at - w.h * head;
+  int lo = 0, hi = items_of(a, w.s) - 1;  // the last item that starts by x
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cost_before(a, w.s, mid) <= x) lo = mid; else hi = mid - 1;
+  }
+  w.p = lo;
+  w.at = at + w.h * head + cost_before(a, w.s, lo);
+}
+
+struct PlanSmem {
+  long long warp_sum[16];
+  long long at;
+  int b;
+};
+
+// Called by all kThreads threads of a CTA: the division of the step and this
+// CTA's walk. False if it has no work.
+template <int kThreads>
+__device__ __forceinline__ bool plan(const PagedArgs &a, PlanSmem &sm,
+                                     Division &d, Walk &w) {
+  static_assert(kThreads % 32 == 0 && kThreads <= 512, "one sum per warp");
+  const int tid = threadIdx.x;
+  const int each = (a.batch + kThreads - 1) / kThreads;
+  const int b0 = min(tid * each, a.batch), b1 = min(b0 + each, a.batch);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += cost_of(a, read_seq(a, b));
+  mine *= a.H_kv;
+  long long upto = mine;  // inclusive prefix within the warp
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    if ((tid & 31) >= o) upto += v;
+  }
+  if ((tid & 31) == 31) sm.warp_sum[tid >> 5] = upto;
+  __syncthreads();
+  long long total = 0, before = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; ++i) {
+    if (i < (tid >> 5)) before += sm.warp_sum[i];
+    total += sm.warp_sum[i];
+  }
+  before += upto - mine;
+  d.total = total;
+  d.ctas = static_cast<int>(
+      min(static_cast<long long>(gridDim.x), max(1ll, total / a.min_piece)));
+  const int c = blockIdx.x;
+  if (total == 0 || c >= d.ctas) return false;
+  w.u0 = d.piece(c);
+  w.u1 = d.piece(c + 1);
+  if (mine > 0 && before <= w.u0 && w.u0 < before + mine) {
+    int b = b0;
+    long long at = before;
+    for (;; ++b) {
+      const long long here = cost_of(a, read_seq(a, b)) * a.H_kv;
+      if (w.u0 < at + here) break;
+      at += here;
+    }
+    sm.b = b;
+    sm.at = at;
+  }
+  __syncthreads();
+  start(a, w, sm.b, sm.at);
+  return true;
+}
+
+// Part of CTA c in the split item `it`: its tiles, none if t0 >= t1.
+__host__ __device__ __forceinline__ void tiles_of_cta(const PagedArgs &a,
+                                             const Division &d, const Part &it,
+                                             int c, int &t0, int &t1) {
+  const long long u0 = d.piece(c), u1 = d.piece(c + 1);
+  t0 = u0 <= it.at ? 0 : tile_at(a, it.tiles, u0 - it.at);
+  t1 = u1 >= it.at + it.cost ? it.tiles : tile_at(a, it.tiles, u1 - it.at);
+}
+
+// Which of its two partial slots a CTA keeps a part in: an item that it does
+// not begin is the first of its piece, one that it does not end the last.
+__host__ __device__ __forceinline__ int slot_of(int t0) { return t0 > 0 ? 0 : 1; }
+
+// A page table entry for the tensor maps: one that is no page reads as the
+// page after the last, which TMA fills with zeros.
+__device__ __forceinline__ int page_entry(const PagedArgs &a, int b, int i) {
+  const int page = a.page_table[b * a.table_stride + i];
+  if (page >= 0 && page < a.num_pages) return page;
+  record_error(FA_ERR_PAGE);
+  return a.num_pages;
+}
+
+// The page that lane `lane` of the producer warp loads for key tile i of a
+// sequence of `keys` rows, and the tile's first row in it; -1: none.
+__device__ __forceinline__ int tile_page(const PagedArgs &a, int b, int keys,
+                                         int i, int lane) {
+  const int row = i * a.tile_keys + (a.page_rows < kTileRows ? lane * a.page_rows : 0);
+  const bool has = a.page_rows < kTileRows
+                       ? lane < a.tile_keys / a.page_rows && row < keys
+                       : lane == 0;
+  return has ? page_entry(a, b, row / a.page_rows) : -1;
+}
+
+}  // namespace paged
+}  // namespace fa

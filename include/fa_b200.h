@@ -539,15 +539,15 @@ int fa_append_paged(const void *q, const int64_t q_strides[2], void *q_out,
  * row r it stands at. One token a sequence is the decode step, a few are
  * drafted tokens being checked, many are a chunk of a prompt; one call takes
  * any mix. q (tokens, H, head_dim) with strides as in fa_append_paged
- * (multiples of 8), o contiguous (tokens, H, head_dim), H % kv_heads == 0
+ * (positive multiples of 8), o contiguous (tokens, H, head_dim), H % kv_heads == 0
  * and H / kv_heads <= 128. Scores, softmax and accumulators are fp32; the
  * probabilities enter the second product in the tensors' 16-bit type. A
  * token that sees no row gets zeros. lse, unless NULL: (tokens, H) fp32, the
  * natural logarithm of each row's sum of exponentials (-inf where it sees
  * no row). Rows of the pages past seq_lens[b] may hold anything.
  * workspace: fa_attend_paged_workspace_bytes() bytes, 16-byte aligned, no
- * initialisation; counters: as for fa_decode, at least as many as the device
- * has SMs. No reference counterpart (its caches are contiguous).
+ * initialisation; counters: as for fa_decode, at least two for each SM of
+ * the device. No reference counterpart (its caches are contiguous).
  */
 size_t fa_attend_paged_workspace_bytes(int head_dim, int device);
 int fa_attend_paged(const void *q, const int64_t q_strides[2], void *o,
