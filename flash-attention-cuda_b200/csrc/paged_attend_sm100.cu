@@ -25,7 +25,7 @@ cudaError_t launch(const PagedArgs &a, int form, const CUtensorMap &tm_q,
                    cudaStream_t stream) {
   if (form == kPagedFew)
     few::attend_few_kernel<D, Dt>
-        <<<sms, few::kThreads, few::Cfg<D>::kSmemBytes, stream>>>(a, tm_k, tm_v);
+        <<<min(sms, few::kMaxGrid), few::kThreads, few::Cfg<D>::kSmemBytes, stream>>>(a, tm_k, tm_v);
   else
     many::attend_many_kernel<D, Dt>
         <<<sms, many::kThreads, many::Cfg<D>::kSmemBytes, stream>>>(a, tm_q, tm_k,
@@ -80,6 +80,10 @@ void attend_paged_plan(PagedArgs &a, int form) {
     a.item_cost = 256;
     a.min_piece = 512;
   }
+#ifdef FA_TUNE
+  if (getenv("FA_COST")) a.item_cost = atoi(getenv("FA_COST"));
+  if (getenv("FA_PIECE")) a.min_piece = atoi(getenv("FA_PIECE"));
+#endif
 }
 
 cudaError_t launch_attend_paged_kernel(const PagedArgs &a, int form,

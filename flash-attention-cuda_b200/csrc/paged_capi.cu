@@ -56,7 +56,8 @@ int check_cache(const fa_paged_cache *c) {
 
 // 4-D view of 16-bit elements (64 of the innermost a box), 128-byte swizzle;
 // what lies outside reads as zero. A dimension of one element takes any
-// stride.
+// stride. Rows that follow one another are fetched into L2 by 256 bytes,
+// rows with others between them by 128, so that nobody else's are.
 int make_map(CUtensorMap *map, const void *base, int dtype, const int (&sizes)[4],
              const int64_t (&strides)[3], int box1, int box3) {
   cuuint64_t dims[4], bytes[3];
@@ -71,7 +72,9 @@ int make_map(CUtensorMap *map, const void *base, int dtype, const int (&sizes)[4
                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                   4, const_cast<void *>(base), dims, bytes, box, step,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  strides[0] == sizes[0] || sizes[0] == 128
+                      ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                      : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
              ? FA_OK
              : FA_EINVAL;

@@ -31,7 +31,9 @@ namespace few {
 
 constexpr int kRows = 16;  // query rows of an item
 constexpr int kWarps = 8;  // consumers
-constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kProducers = 2;  // one warp for K, one for V
+constexpr int kThreads = 32 * (kWarps + kProducers);
+constexpr int kMaxGrid = 160;  // CTAs (statistics of a join in shared memory)
 constexpr float kNegBig = -1e30f;  // the maximum of no scores yet
 
 template <int D>
@@ -40,31 +42,22 @@ struct Cfg {
   static constexpr uint32_t kTile = D / 64 * kHalf;    // K or V
   static constexpr uint32_t kStage = 2 * kTile;
   static constexpr int kStages = 6 * 64 / D;           // 192 KiB
-  static constexpr int kChunk = 32;  // dims joined at a time
+  // The warps' states at the end of a part: O, 16 KiB at a time, then (m, l)
   static constexpr uint32_t kRedOff = kStages * kStage;
-  static constexpr uint32_t kRedBytes = kWarps * kRows * kChunk * 4;
-  static constexpr uint32_t kStatOff = kRedOff + kRedBytes;  // (m, l) per warp, row
+  static constexpr uint32_t kRedBytes = 16384;
+  static constexpr uint32_t kStatOff = kRedOff + kRedBytes;  // per warp and row
   static constexpr uint32_t kStatBytes = kWarps * kRows * 8;
   static constexpr uint32_t kBarOff = kStatOff + kStatBytes;
-  // full[stage], empty[stage], consumers
-  static constexpr uint32_t kMiscOff = kBarOff + (2 * kStages + 1) * 8;
+  // full[stage], empty[stage]
+  static constexpr uint32_t kMiscOff = kBarOff + 2 * kStages * 8;
   static constexpr uint32_t kSmemBytes = kMiscOff + sizeof(PlanSmem) + 16;
   static_assert(kSmemBytes + 1024 <= 228 * 1024, "above the SM's shared memory");
   static constexpr int kSlotFloats = kRows * (D + 2);  // a partial: O, m, l
 };
 
-// A bounded barrier of the consumer warps.
-struct Sync {
-  uint64_t *bar;
-  uint32_t phase = 0;
-  __device__ __forceinline__ bool operator()() {
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-    const bool ok = mbar_wait(bar, phase);
-    phase ^= 1;
-    return ok;
-  }
-};
+// Barrier of the consumer warps. A warp whose wait ran out goes on through
+// the barriers without waiting for tiles again, so nobody is left behind.
+__device__ __forceinline__ void meet() { named_bar_sync(1, 32 * kWarps); }
 
 // Row r of an item: new token r / group of it, head r % group of the group.
 struct Row {
@@ -95,83 +88,120 @@ __device__ __forceinline__ void store_result(const PagedArgs &a, const Row &w,
     a.lse[row] = l == 0.f ? -INFINITY : 0.69314718055994531f * (m + log2f(l));
 }
 
-// Joins the partials of a split item (by the CTA that finished last).
+// Joins the partials of a split item (by the CTA that finished last): the
+// CTAs' maxima and sums become weights in shared memory first, then every
+// thread adds up one row's four dims over every n-th CTA, so that all loads
+// of a step are under way together.
 template <int D>
-__device__ __forceinline__ bool join(const PagedArgs &a, const Division &d,
+__device__ __forceinline__ void join(const PagedArgs &a, const Division &d,
                                      const Part &it, int n_rows, float *red,
-                                     Sync &sync, int dtype) {
+                                     int dtype) {
   using C = Cfg<D>;
   const int tid = threadIdx.x;  // 256 consumers
-  const int c0 = d.owner(it.at), c1 = d.owner(it.at + it.cost - 1);
-  // groups of threads share a row's dims; the groups take every n-th CTA
+  const int c0 = d.owner(it.at), n = d.owner(it.at + it.cost - 1) - c0 + 1;
+  // red: weight [CTA][row], sum and maximum per row, the CTAs' slots (-1:
+  // none of the item); later the sums of the thread groups
+  float *weight = red;
+  float2 *total = reinterpret_cast<float2 *>(red + kMaxGrid * kRows);
+  int *slots = reinterpret_cast<int *>(total + kRows);
+  static_assert((kMaxGrid * kRows + 2 * kRows + kMaxGrid) * 4 <= C::kRedBytes,
+                "the join's statistics fit");
   const int units = n_rows * (D / 4);
   const int groups = max(1, 32 * kWarps / units);
+  if (tid < n) {
+    int t0, t1;
+    tiles_of_cta(a, d, it, c0 + tid, t0, t1);
+    slots[tid] = t0 < t1 ? 2 * (c0 + tid) + slot_of(t0) : -1;
+  }
+  meet();
+  {
+    // sixteen threads a row
+    constexpr int kMost = (kMaxGrid + 15) / 16;
+    const int row = tid >> 4;
+    float m[kMost], l[kMost];
+    float M = kNegBig, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+      const int c = (tid & 15) + 16 * i;
+      const int slot = c < n && row < n_rows ? slots[c] : -1;
+      const float *p = a.partials + slot * C::kSlotFloats + kRows * D + row;
+      m[i] = slot >= 0 ? __ldcg(p) : kNegBig;
+      l[i] = slot >= 0 ? __ldcg(p + kRows) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+      if (l[i] == 0.f) m[i] = kNegBig;  // saw nothing
+      M = fmaxf(M, m[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1)
+      M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+      const int c = (tid & 15) + 16 * i;
+      const float w = l[i] == 0.f ? 0.f : fast_exp2(m[i] - M);
+      if (c < n) weight[c * kRows + row] = w;
+      L = fmaf(l[i], w, L);
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if ((tid & 15) == 0) total[row] = make_float2(M, L);
+  }
+  meet();
   for (int u0 = 0; u0 < units; u0 += 32 * kWarps) {
     const int g = groups > 1 ? tid / units : 0;
     const int u = groups > 1 ? tid % units : u0 + tid;
     const bool on = g < groups && u < units;
-    const int row = u / (D / 4), d4 = u % (D / 4);
-    float m = kNegBig, l = 0.f;
+    const int row = on ? u / (D / 4) : 0, d4 = u % (D / 4);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (on) {
-#pragma unroll 4
-      for (int c = c0 + g; c <= c1; c += groups) {
-        int t0, t1;
-        tiles_of_cta(a, d, it, c, t0, t1);
-        if (t0 >= t1) continue;
-        const float *p = a.partials +
-                         (2 * static_cast<size_t>(c) + slot_of(t0)) * C::kSlotFloats;
-        const float mc = __ldcg(p + kRows * D + row);
-        const float lc = __ldcg(p + kRows * D + kRows + row);
-        const float4 oc = __ldcg(reinterpret_cast<const float4 *>(p + row * D) + d4);
-        if (lc == 0.f) continue;  // saw nothing
-        const float mn = fmaxf(m, mc);
-        const float s0 = fast_exp2(m - mn), s1 = fast_exp2(mc - mn);
-        m = mn;
-        l = l * s0 + lc * s1;
-        acc.x = acc.x * s0 + oc.x * s1;
-        acc.y = acc.y * s0 + oc.y * s1;
-        acc.z = acc.z * s0 + oc.z * s1;
-        acc.w = acc.w * s0 + oc.w * s1;
+    constexpr int kBatch = 16;  // loads under way
+    for (int c1 = on ? g : n; c1 < n; c1 += kBatch * groups) {
+      float4 o[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int c = c1 + i * groups;
+        const int slot = c < n ? slots[c] : -1;
+        o[i] = slot >= 0 ? __ldcg(reinterpret_cast<const float4 *>(
+                               a.partials + slot * C::kSlotFloats + row * D) + d4)
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int c = c1 + i * groups;
+        const float w = c < n ? weight[c * kRows + row] : 0.f;
+        acc.x = fmaf(o[i].x, w, acc.x);
+        acc.y = fmaf(o[i].y, w, acc.y);
+        acc.z = fmaf(o[i].z, w, acc.z);
+        acc.w = fmaf(o[i].w, w, acc.w);
       }
     }
+    const float2 ml = total[row];
     if (groups > 1) {
-      float *mine = red + tid * 6;
-      mine[0] = m;
-      mine[1] = l;
-      mine[2] = acc.x;
-      mine[3] = acc.y;
-      mine[4] = acc.z;
-      mine[5] = acc.w;
-      if (!sync()) return false;
+      meet();  // the weights have been read
+      float4 *sums = reinterpret_cast<float4 *>(red);
+      sums[tid] = acc;
+      meet();
       if (on && g == 0) {
         for (int o = 1; o < groups; ++o) {
-          const float *p = red + (tid + o * units) * 6;
-          if (p[1] == 0.f) continue;
-          const float mn = fmaxf(m, p[0]);
-          const float s0 = fast_exp2(m - mn), s1 = fast_exp2(p[0] - mn);
-          m = mn;
-          l = l * s0 + p[1] * s1;
-          acc.x = acc.x * s0 + p[2] * s1;
-          acc.y = acc.y * s0 + p[3] * s1;
-          acc.z = acc.z * s0 + p[4] * s1;
-          acc.w = acc.w * s0 + p[5] * s1;
+          const float4 v = sums[tid + o * units];
+          acc.x += v.x;
+          acc.y += v.y;
+          acc.z += v.z;
+          acc.w += v.w;
         }
       }
     }
     if (on && g == 0) {
       const Row w = row_of(a, it, row);
-      store_result<D>(a, w, 4 * d4, make_float2(acc.x, acc.y), m, l, dtype);
-      store_result<D>(a, w, 4 * d4 + 2, make_float2(acc.z, acc.w), m, l, dtype);
+      store_result<D>(a, w, 4 * d4, make_float2(acc.x, acc.y), ml.x, ml.y, dtype);
+      store_result<D>(a, w, 4 * d4 + 2, make_float2(acc.z, acc.w), ml.x, ml.y, dtype);
     }
   }
-  return sync();  // red is free again
 }
 
 template <int D, typename Dt>
 __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
-                        uint8_t *smem, uint64_t *full, uint64_t *empty,
-                        Sync sync) {
+                        uint8_t *smem, uint64_t *full, uint64_t *empty) {
   using C = Cfg<D>;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -183,6 +213,7 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
   int *last = reinterpret_cast<int *>(smem + C::kMiscOff + sizeof(PlanSmem));
 
   int pos = 0;  // ring position
+  bool ok = true;
   Part it;
   while (walk.next(a, it)) {
     const Row w0 = row_of(a, it, quad), w1 = row_of(a, it, quad + 8);
@@ -209,7 +240,11 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
 
     for (int i = it.t0; i < it.t1; ++i, ++pos) {
       const int slot = pos % C::kStages;
-      if (!mbar_wait(&full[slot], (pos / C::kStages) & 1)) return;
+      if (!ok || !mbar_wait(&full[slot], (pos / C::kStages) & 1)) {
+        ok = false;
+        break;
+      }
+      if (threadIdx.x == 0 && pos == 0) FA_TRACE_CTA(2);
       const int base = i * a.tile_keys;
       // rows of this warp that the tile holds
       const int here = min(it.keys - base, a.tile_keys) - key0;
@@ -297,6 +332,7 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
     }
 
     // ---- the warps' states, joined
+    if (threadIdx.x == 0) FA_TRACE_CTA(3);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
@@ -305,50 +341,43 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
       stat[warp * kRows + quad] = make_float2(m0, l0);
       stat[warp * kRows + quad + 8] = make_float2(m1, l1);
     }
-    if (!sync()) return;
-    float M0 = kNegBig, M1 = kNegBig;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      M0 = fmaxf(M0, stat[i * kRows + quad].x);
-      M1 = fmaxf(M1, stat[i * kRows + quad + 8].x);
-    }
-    const float f0 = fast_exp2(m0 - M0), f1 = fast_exp2(m1 - M1);
     const int group = a.H / a.H_kv;
     const int n_rows = min(a.item_tokens, it.seq.n - it.token) * group;
     float *slot = a.partials + (2 * static_cast<size_t>(blockIdx.x) +
                                 slot_of(it.t0)) * C::kSlotFloats;
     const bool whole = it.whole();
+    // as many dims at a time as fit for this many rows: a power of two, 32
+    // at 16 rows, all of them up to 4 rows of 128 or 8 of 64
+    const int chunk = min(D, 32 << (n_rows <= 4 ? 2 : n_rows <= 8 ? 1 : 0));
+    for (int d0 = 0; d0 < D; d0 += chunk) {
 #pragma unroll
-    for (int ch = 0; ch < D / C::kChunk; ++ch) {
-      constexpr int kDt = C::kChunk / 8;
-#pragma unroll
-      for (int e = 0; e < kDt; ++e) {
-        const int dt = ch * kDt + e;
-        float *r = red + (warp * kRows + quad) * C::kChunk + 8 * e + 2 * qid;
+      for (int dt = 0; dt < D / 8; ++dt) {
+        if (8 * dt < d0 || 8 * dt >= d0 + chunk) continue;
+        float *r = red + (warp * n_rows + quad) * chunk + 8 * dt - d0 + 2 * qid;
         if (quad < n_rows)
-          *reinterpret_cast<float2 *>(r) = make_float2(o[dt][0] * f0, o[dt][1] * f0);
+          *reinterpret_cast<float2 *>(r) = make_float2(o[dt][0], o[dt][1]);
         if (quad + 8 < n_rows)
-          *reinterpret_cast<float2 *>(r + 8 * C::kChunk) =
-              make_float2(o[dt][2] * f1, o[dt][3] * f1);
+          *reinterpret_cast<float2 *>(r + 8 * chunk) = make_float2(o[dt][2], o[dt][3]);
       }
-      if (!sync()) return;
-      // thread: row tid / 16, dims 2 (tid % 16) (+1) of the chunk
-      const int r = threadIdx.x >> 4, c = 2 * (threadIdx.x & 15);
-      if (r < n_rows) {
+      meet();
+      for (int e = threadIdx.x; e < n_rows * (chunk / 2); e += 32 * kWarps) {
+        const int r = e / (chunk / 2), c = 2 * (e - r * (chunk / 2));
+        float M = kNegBig;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) M = fmaxf(M, stat[i * kRows + r].x);
         float2 sum = make_float2(0.f, 0.f);
-        float M = kNegBig, L = 0.f;
+        float L = 0.f;
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) {
+          const float2 ml = stat[i * kRows + r];
           const float2 v = *reinterpret_cast<const float2 *>(
-              red + (i * kRows + r) * C::kChunk + c);
-          sum.x += v.x;
-          sum.y += v.y;
-          M = fmaxf(M, stat[i * kRows + r].x);
+              red + (i * n_rows + r) * chunk + c);
+          const float w = fast_exp2(ml.x - M);
+          sum.x = fmaf(v.x, w, sum.x);
+          sum.y = fmaf(v.y, w, sum.y);
+          L = fmaf(ml.y, w, L);
         }
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i)
-          L += stat[i * kRows + r].y * fast_exp2(stat[i * kRows + r].x - M);
-        const int dim = ch * C::kChunk + c;
+        const int dim = d0 + c;
         if (whole) {
           store_result<D>(a, row_of(a, it, r), dim, sum, M, L, Dt::kDtype);
         } else {
@@ -359,9 +388,10 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
           }
         }
       }
-      if (!whole && ch == D / C::kChunk - 1) __threadfence();
-      if (!sync()) return;
+      if (!whole && d0 + chunk == D) __threadfence();
+      meet();
     }
+    if (threadIdx.x == 0) FA_TRACE_CTA(4);
     if (!whole) {
       // the part that completes the item's tiles joins them
       uint32_t *counter = a.counters + d.owner(it.at);
@@ -371,9 +401,11 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
         if (*last) *counter = 0;
         __threadfence();
       }
-      if (!sync()) return;
-      if (*last && !join<D>(a, d, it, n_rows, red, sync, Dt::kDtype)) return;
-      if (!sync()) return;
+      meet();
+      if (threadIdx.x == 0) FA_TRACE_CTA(5);
+      if (*last) join<D>(a, d, it, n_rows, red, Dt::kDtype);
+      if (threadIdx.x == 0) FA_TRACE_CTA(6);
+      meet();
     }
   }
 }
@@ -388,34 +420,39 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lane = threadIdx.x & 31;
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::kBarOff);
   uint64_t *empty = full + C::kStages;
-  uint64_t *consumers = empty + C::kStages;
   PlanSmem *ps = reinterpret_cast<PlanSmem *>(smem + C::kMiscOff);
-  int *failed = reinterpret_cast<int *>(smem + C::kMiscOff + sizeof(PlanSmem)) + 1;
+  if (threadIdx.x == 0) FA_TRACE_CTA(0);
+#ifdef FA_TRACE
+  if (threadIdx.x == 0) { uint32_t sm; asm volatile("mov.u32 %0, %%smid;" : "=r"(sm)); g_fa_trace[blockIdx.x * 8 + 7] = sm; }
+#endif
   if (smem_u32(smem) & 1023u) {
     if (threadIdx.x == 0) record_error(FA_ERR_SMEM_ALIGN);
     return;
   }
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kWarps);
-    }
-    mbar_init(consumers, kWarps);
-    fence_barrier_init();
-    prefetch_tensormap(&tm_k);
-    prefetch_tensormap(&tm_v);
-    *failed = device_failed();
-  }
   Division d;
   Walk walk;
-  if (!plan<kThreads>(a, *ps, d, walk)) return;  // synchronises the CTA
-  if (*failed) return;
+  const bool work = plan<kThreads>(a, *ps, d, walk, [&] {
+    if (warp == kWarps && lane == 0) {
+      for (int s = 0; s < C::kStages; ++s) {
+        mbar_init(&full[s], kProducers);
+        mbar_init(&empty[s], kWarps);
+      }
+      fence_barrier_init();
+      prefetch_tensormap(&tm_k);
+      prefetch_tensormap(&tm_v);
+    }
+  });
+  if (!work) return;
+  if (threadIdx.x == 0) FA_TRACE_CTA(1);
 
   if (warp < kWarps) {
-    consume<D, Dt>(a, d, walk, smem, full, empty, Sync{consumers});
+    consume<D, Dt>(a, d, walk, smem, full, empty);
     return;
   }
-  // ---- producer: lane j loads page j of the tile
+  // ---- producers, one of K and one of V (small pages make many boxes, and
+  // a warp issues one in 50 ns): lane j loads page j of the tile
+  const bool is_v = warp > kWarps;
+  const CUtensorMap *map = is_v ? &tm_v : &tm_k;
   const int box = min(a.page_rows, kTileRows);
   int pos = 0;
   bool ok = true;
@@ -431,17 +468,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const uint32_t pages = __ballot_sync(0xffffffffu, page >= 0);
       if (lane == 0)
-        mbar_arrive_expect_tx(&full[slot], __popc(pages) * box * 128 * (D / 64) * 2);
+        mbar_arrive_expect_tx(&full[slot], __popc(pages) * box * 128 * (D / 64));
       __syncwarp();
       if (page >= 0) {
         const int row = a.page_rows < kTileRows ? 0 : i * a.tile_keys % a.page_rows;
-        uint8_t *to = smem + slot * C::kStage + lane * box * 128;
+        uint8_t *to = smem + slot * C::kStage + (is_v ? C::kTile : 0) + lane * box * 128;
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h) {
-          tma_load_4d(to + h * C::kHalf, &tm_k, &full[slot], 64 * h, row, it.h, page);
-          tma_load_4d(to + C::kTile + h * C::kHalf, &tm_v, &full[slot], 64 * h, row,
-                      it.h, page);
-        }
+        for (int h = 0; h < D / 64; ++h)
+          tma_load_4d(to + h * C::kHalf, map, &full[slot], 64 * h, row, it.h, page);
       }
       page = next;
     }

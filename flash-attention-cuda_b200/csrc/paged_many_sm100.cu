@@ -16,9 +16,11 @@
 //
 // CTA = 12 warps:
 //   0-3 / 4-7  softmax of query tile 0 / 1 (thread = row = TMEM lane)
-//   8          TMA producer: lane j loads page j of a key tile
+//   8, 10      TMA producers of Q and K, and of V: lane j loads page j of a
+//              key tile (a warp issues a box in 50 ns, and small pages make
+//              many)
 //   9          MMA issuer (one elected thread); owns the TMEM allocation
-//   10-11      idle (they give their registers to the softmax warps)
+//   11         walks the CTA's parts and hands them to the others
 //
 // Shared memory: Q_t (128 rows x D), then a ring of key tiles (K and V, 128
 // rows x D each: 2 at D 128, 5 at 64), rows as 128-byte-swizzled halves of
@@ -41,8 +43,11 @@ namespace many {
 
 constexpr int kRows = 128;  // query rows of a tile
 constexpr int kThreads = 384;
-constexpr int kProducerWarp = 8;
+constexpr int kProducerWarp = 8;   // Q, K
 constexpr int kMmaWarp = 9;
+constexpr int kProducerWarpV = 10;
+constexpr int kWalkWarp = 11;
+constexpr int kParts = 4;  // parts handed out ahead
 constexpr int kCtrlRegs = 24;
 constexpr int kSoftmaxRegs = 240;
 static_assert(128 * kCtrlRegs + 256 * kSoftmaxRegs <= kThreads * 168,
@@ -69,11 +74,13 @@ struct Cfg {
   static constexpr int kPFull = kSFull + 2;          // + tile
   static constexpr int kODone = kPFull + 2;          // + tile
   static constexpr int kJoin = kODone + 2;           // + tile
-  static constexpr int kDrain = kJoin + 2;
+  static constexpr int kPartFull = kJoin + 2;        // + slot
+  static constexpr int kPartEmpty = kPartFull + kParts;  // + slot
+  static constexpr int kDrain = kPartEmpty + kParts;
   static constexpr int kBars = kDrain + 1;
   static constexpr uint32_t kMiscOff = kBarOff + kBars * 8;
-  // plan, TMEM address, abort flag, per-tile join flags
-  static constexpr uint32_t kSmemBytes = kMiscOff + sizeof(PlanSmem) + 32;
+  static constexpr uint32_t kCtrlOff = kMiscOff + sizeof(PlanSmem);
+  static constexpr uint32_t kSmemBytes = kCtrlOff + 512;
   static_assert(kSmemBytes + 1024 <= 228 * 1024, "above the SM's shared memory");
   static constexpr uint32_t kTmemO = 256;  // + D * tile
   // a partial of one tile: O as [D / 4][row] float4, then m and l per row
@@ -112,41 +119,105 @@ __device__ __forceinline__ uint64_t v_desc(uint32_t addr) {
          (static_cast<uint64_t>(Cfg<D>::kHalf >> 4) << 16);
 }
 
-// Tokens of a tile, and the end of tile t's key tiles within a part (its
-// start if the tile has no token or no key there).
-__device__ __forceinline__ int tile_tokens(const PagedArgs &a) {
-  return a.item_tokens / 2;
-}
-__device__ __forceinline__ int tile_end(const PagedArgs &a, const Part &it, int t) {
-  const int first = it.token + t * tile_tokens(a);
-  const int last = min(first + tile_tokens(a), it.seq.n) - 1;
-  if (last < first) return it.t0;
-  const int tiles = (rows_seen(a, it.seq, last) + a.tile_keys - 1) / a.tile_keys;
-  return max(it.t0, min(it.t1, tiles));
-}
+// A part as the CTA's warps see it.
+struct Job {
+  int b, h;        // sequence (-1: no more parts), K/V head
+  int token;       // first packed token
+  int n;           // tokens of the item
+  int row0;        // cache row that the first stands at
+  int keys;        // rows of the sequence in the cache
+  int tiles, t0, t1;  // key tiles of the item and of this part
+  int end[2];      // of t0 .. t1, where each query tile's end
+  long long at, cost;
+  __device__ bool whole() const { return t0 == 0 && t1 == tiles; }
+};
 
 struct Ctrl {
   uint32_t tmem;
   volatile uint32_t abort;
-  uint32_t join[2];
+  volatile uint32_t join[2];
+  Division division;
+  Job job[kParts];
 };
 
+__device__ __forceinline__ int tile_tokens(const PagedArgs &a) {
+  return a.item_tokens / 2;
+}
+__device__ __forceinline__ int job_seen(const PagedArgs &a, const Job &j, int token) {
+  return a.causal ? min(max(j.row0 + token + 1, 0), j.keys) : j.keys;
+}
+
+// The n-th part, once it is there (null if the wait ran out); to be released
+// by every warp.
 template <int D>
-__device__ void produce(const PagedArgs &a, Walk &walk, uint8_t *smem,
-                        uint64_t *bars, Ctrl *ctrl, const CUtensorMap *tm_q,
-                        const CUtensorMap *tm_k, const CUtensorMap *tm_v) {
+__device__ __forceinline__ const Job *take(Ctrl *ctrl, uint64_t *bars, int n) {
+  using C = Cfg<D>;
+  if (!mbar_wait(&bars[C::kPartFull + n % kParts], (n / kParts) & 1)) {
+    ctrl->abort = 1;
+    return nullptr;
+  }
+  return &ctrl->job[n % kParts];
+}
+template <int D>
+__device__ __forceinline__ void release(uint64_t *bars, int n) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&bars[Cfg<D>::kPartEmpty + n % kParts]);
+}
+
+template <int D>
+__device__ void hand_out(const PagedArgs &a, Walk &walk, uint64_t *bars, Ctrl *ctrl) {
+  using C = Cfg<D>;
+  for (int n = 0;; ++n) {
+    Part it;
+    const bool more = walk.next(a, it);
+    if (n >= kParts && !mbar_wait(&bars[C::kPartEmpty + n % kParts], (n / kParts - 1) & 1)) {
+      ctrl->abort = 1;
+      return;
+    }
+    Job &j = ctrl->job[n % kParts];
+    j.b = more ? it.b : -1;
+    if (more) {
+      j.h = it.h;
+      j.token = it.seq.lo + it.token;
+      j.n = min(a.item_tokens, it.seq.n - it.token);
+      j.row0 = static_cast<int>(max(it.seq.len - it.seq.n + it.token, -(1ll << 31)));
+      j.keys = it.keys;
+      j.tiles = it.tiles;
+      j.t0 = it.t0;
+      j.t1 = it.t1;
+      j.at = it.at;
+      j.cost = it.cost;
+      for (int t = 0; t < 2; ++t) {
+        const int last = min(j.n, (t + 1) * tile_tokens(a)) - 1;
+        const int end = last < t * tile_tokens(a)
+                            ? 0 : (job_seen(a, j, last) + a.tile_keys - 1) / a.tile_keys;
+        j.end[t] = max(it.t0, min(it.t1, end));
+      }
+    }
+    mbar_arrive(&bars[C::kPartFull + n % kParts]);
+    if (!more) return;
+  }
+}
+
+template <int D, bool kV>
+__device__ void produce(const PagedArgs &a, uint8_t *smem, uint64_t *bars,
+                        Ctrl *ctrl, const CUtensorMap *tm_q, const CUtensorMap *tm) {
   using C = Cfg<D>;
   const int lane = threadIdx.x & 31;
-  const int group = a.H / a.H_kv;
   const int box = min(a.page_rows, kTileRows);
   int pos = 0, q_used[2] = {0, 0};
   uint32_t tail_phase = 0;
   bool ok = true;
-  Part it;
-  while (ok && walk.next(a, it)) {
-    int page = it.t0 < it.t1 ? tile_page(a, it.b, it.keys, it.t0, lane) : -1;
-    for (int t = 0; ok && t < 2; ++t) {
-      if (tile_end(a, it, t) <= it.t0) continue;
+  for (int n = 0; ok; ++n) {
+    const Job *job = take<D>(ctrl, bars, n);
+    if (!job || job->b < 0) break;
+    const int b = job->b, h = job->h, keys = job->keys, t0 = job->t0, t1 = job->t1;
+    const int token = job->token;
+    const bool has[2] = {job->end[0] > t0, job->end[1] > t0};
+    release<D>(bars, n);
+    int page = t0 < t1 ? tile_page(a, b, keys, t0, lane) : -1;
+    for (int t = 0; !kV && ok && t < 2; ++t) {
+      if (!has[t]) continue;
       if (q_used[t] > 0 && !mbar_wait(&bars[C::kQEmpty + t], (q_used[t] - 1) & 1)) {
         ok = false;
         break;
@@ -154,47 +225,45 @@ __device__ void produce(const PagedArgs &a, Walk &walk, uint8_t *smem,
       ++q_used[t];
       if (lane == 0) {
         uint64_t *bar = &bars[C::kQFull + t];
-        mbar_arrive_expect_tx(bar, tile_tokens(a) * group * 128 * (D / 64));
-        for (int h = 0; h < D / 64; ++h)
-          tma_load_4d(smem + C::kQOff + t * C::kTile + h * C::kHalf, tm_q, bar,
-                      64 * h, 0, it.h, it.seq.lo + it.token + t * tile_tokens(a));
+        mbar_arrive_expect_tx(bar, tile_tokens(a) * (a.H / a.H_kv) * 128 * (D / 64));
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_4d(smem + C::kQOff + t * C::kTile + c * C::kHalf, tm_q, bar,
+                      64 * c, 0, h, token + t * tile_tokens(a));
       }
     }
-    for (int i = it.t0; ok && i < it.t1; ++i, ++pos) {
-      const int next = i + 1 < it.t1 ? tile_page(a, it.b, it.keys, i + 1, lane) : -1;
+    for (int i = t0; ok && i < t1; ++i, ++pos) {
+      const int next = i + 1 < t1 ? tile_page(a, b, keys, i + 1, lane) : -1;
       const int slot = pos % C::kStages, use = pos / C::kStages;
       if (ctrl->abort ||
           (use > 0 && !mbar_wait(&bars[C::kEmpty + slot], (use - 1) & 1))) {
         ok = false;
         break;
       }
-      // A tile that reaches past the sequence's rows goes through a barrier
-      // of its own: its V rows there may hold anything, NaN included, and are
+      // A V tile that reaches past the sequence's rows goes through a barrier
+      // of its own: the rows there may hold anything, NaN included, and are
       // cleared before the tile is handed on (P is zero there, and zero times
       // NaN is not).
-      const int valid = it.keys - i * a.tile_keys;
-      const bool tail = valid < a.tile_keys;
+      const int valid = keys - i * a.tile_keys;
+      const bool tail = kV && valid < a.tile_keys;
       uint64_t *bar = &bars[tail ? C::kTail : C::kFull + slot];
       const uint32_t pages = __ballot_sync(0xffffffffu, page >= 0);
       if (lane == 0)
-        mbar_arrive_expect_tx(bar, __popc(pages) * box * 128 * (D / 64) * 2);
+        mbar_arrive_expect_tx(bar, __popc(pages) * box * 128 * (D / 64));
       __syncwarp();
-      uint8_t *stage = smem + C::kRingOff + slot * C::kStage;
+      uint8_t *tile = smem + C::kRingOff + slot * C::kStage + (kV ? C::kTile : 0);
       if (page >= 0) {
         const int row = a.page_rows < kTileRows ? 0 : i * a.tile_keys % a.page_rows;
-        uint8_t *to = stage + lane * box * 128;
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h) {
-          tma_load_4d(to + h * C::kHalf, tm_k, bar, 64 * h, row, it.h, page);
-          tma_load_4d(to + C::kTile + h * C::kHalf, tm_v, bar, 64 * h, row, it.h, page);
-        }
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_4d(tile + lane * box * 128 + c * C::kHalf, tm, bar, 64 * c, row, h,
+                      page);
       }
       if (tail) {
         ok = mbar_wait(bar, tail_phase);
         tail_phase ^= 1;
-        for (int h = 0; h < D / 64; ++h)
+        for (int c = 0; c < D / 64; ++c)
           for (int e = valid * 8 + lane; e < a.tile_keys * 8; e += 32)
-            *reinterpret_cast<uint4 *>(stage + C::kTile + h * C::kHalf + 16 * e) =
+            *reinterpret_cast<uint4 *>(tile + c * C::kHalf + 16 * e) =
                 make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
         __syncwarp();
@@ -203,7 +272,7 @@ __device__ void produce(const PagedArgs &a, Walk &walk, uint8_t *smem,
       page = next;
     }
   }
-  if (!ok) {
+  if (!ok || ctrl->abort) {
     ctrl->abort = 1;
     // no copy of ours may still be landing when the CTA exits
     for (int t = 0; t < 2; ++t)
@@ -214,8 +283,7 @@ __device__ void produce(const PagedArgs &a, Walk &walk, uint8_t *smem,
 }
 
 template <int D, typename Dt>
-__device__ void issue(const PagedArgs &a, Walk &walk, uint8_t *smem,
-                      uint64_t *bars, Ctrl *ctrl) {
+__device__ void issue(const PagedArgs &a, uint8_t *smem, uint64_t *bars, Ctrl *ctrl) {
   using C = Cfg<D>;
   const bool leader = elect_one();
   const uint32_t tmem = __shfl_sync(0xffffffffu, ctrl->tmem, 0);
@@ -234,13 +302,16 @@ __device__ void issue(const PagedArgs &a, Walk &walk, uint8_t *smem,
   int q_used[2] = {0, 0};     // queries taken
   int done[2] = {0, 0};       // P V products issued
   bool ok = true;
-  Part it;
-  while (ok && walk.next(a, it)) {
-    if (it.t0 >= it.t1) continue;
-    const int end[2] = {tile_end(a, it, 0), tile_end(a, it, 1)};
+  for (int n = 0; ok; ++n) {
+    const Job *job = take<D>(ctrl, bars, n);
+    if (!job || job->b < 0) break;
+    const int t0 = job->t0, t1 = job->t1;
+    const int end[2] = {job->end[0], job->end[1]};
+    release<D>(bars, n);
+    if (t0 >= t1) continue;
     // first S of each tile; its tensor memory was P of the last item
     for (int t = 0; ok && t < 2; ++t) {
-      if (end[t] <= it.t0) continue;
+      if (end[t] <= t0) continue;
       ok = mbar_wait(&bars[C::kQFull + t], q_used[t] & 1) &&
            mbar_wait(&bars[C::kFull + pos % C::kStages], (pos / C::kStages) & 1) &&
            (done[t] == 0 || mbar_wait(&bars[C::kODone + t], (done[t] - 1) & 1));
@@ -248,10 +319,10 @@ __device__ void issue(const PagedArgs &a, Walk &walk, uint8_t *smem,
       ++q_used[t];
       tc_fence_after();
       s_tile(t, pos);
-      if (leader && end[t] == it.t0 + 1) mma_commit(&bars[C::kQEmpty + t]);
+      if (leader && end[t] == t0 + 1) mma_commit(&bars[C::kQEmpty + t]);
       __syncwarp();
     }
-    for (int j = it.t0; ok && j < it.t1; ++j, ++pos) {
+    for (int j = t0; ok && j < t1; ++j, ++pos) {
       if (ctrl->abort) {
         ok = false;
         break;
@@ -268,7 +339,7 @@ __device__ void issue(const PagedArgs &a, Walk &walk, uint8_t *smem,
         if (leader) {
           issue_pv<D, Dt>(tmem + C::kTmemO + D * t, tmem + 128 * t,
                           vdesc0 + ((C::kRingOff + slot * C::kStage + C::kTile) >> 4),
-                          j > it.t0);
+                          j > t0);
           mma_commit(&bars[C::kODone + t]);
           // the last product of the key tile frees its stage
           if (t == 1 || j >= end[1]) mma_commit(&bars[C::kEmpty + slot]);
@@ -335,9 +406,9 @@ __device__ __forceinline__ void store_dims(__half *dst, const uint32_t (&o)[32],
   }
 }
 
+// One query tile's softmax and results. Returns false if a wait ran out.
 template <int D, typename Dt>
-__device__ void soften(const PagedArgs &a, const Division &d, Walk &walk,
-                       uint64_t *bars, Ctrl *ctrl) {
+__device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
   using C = Cfg<D>;
   const int warp = threadIdx.x >> 5;
   const int t = warp >> 2;
@@ -346,31 +417,40 @@ __device__ void soften(const PagedArgs &a, const Division &d, Walk &walk,
   const uint32_t tS = ctrl->tmem + lane_addr + 128 * t;
   const uint32_t tO = ctrl->tmem + lane_addr + C::kTmemO + D * t;
   const int group = a.H / a.H_kv;
-  const int tok = row / group;  // token of this row within its tile
-  int done = 0;                 // key tiles of this query tile so far
+  // this row's token within the item, -1 for none (the tile's last rows where
+  // the group does not divide it)
+  const int tok = row / group < tile_tokens(a) ? t * tile_tokens(a) + row / group : -1;
+  int done = 0;  // key tiles of this query tile so far
   uint32_t met = 0;
-  Part it;
-  while (walk.next(a, it)) {
-    const int token = it.token + t * tile_tokens(a) + tok;
-    const bool real = tok < tile_tokens(a) && token < it.seq.n;
-    const int seen = real ? rows_seen(a, it.seq, token) : 0;
-    const int end = tile_end(a, it, t);
+  // the tile's 128 threads meet (bounded, like every wait here)
+  auto meet = [&]() {
+    mbar_arrive(&bars[C::kJoin + t]);
+    const bool ok = mbar_wait(&bars[C::kJoin + t], met & 1);
+    ++met;
+    return ok;
+  };
+  for (int n = 0;; release<D>(bars, n), ++n) {
+    const Job *job = take<D>(ctrl, bars, n);
+    if (!job) return false;
+    if (job->b < 0) return true;
+    const int t0 = job->t0, end = job->end[t];
+    const bool real = tok >= 0 && tok < job->n;
+    const int seen = real ? job_seen(a, *job, tok) : 0;
     // a warp without a row only keeps the tile's barriers going
     const bool idle = !__any_sync(0xffffffffu, real);
     // keys that every row of the tile sees
-    const int all_see = rows_seen(a, it.seq, it.token + t * tile_tokens(a));
+    const int all_see =
+        a.tile_keys < kTileRows ? -1 : job_seen(a, *job, t * tile_tokens(a));
     float m = -INFINITY, l = 0.f;
 
-    for (int j = it.t0; j < end; ++j, ++done) {
-      if (ctrl->abort || !mbar_wait(&bars[C::kSFull + t], done & 1)) {
-        ctrl->abort = 1;
-        return;
-      }
+    for (int j = t0; j < end; ++j, ++done) {
+      if (ctrl->abort || !mbar_wait(&bars[C::kSFull + t], done & 1)) return false;
       if (idle) {
         mbar_arrive(&bars[C::kPFull + t]);
         continue;
       }
       tc_fence_after();
+      if (threadIdx.x == 0 && done == 0) FA_TRACE_CTA(2);
       uint32_t sr[4][32];
       tmem_ld32(tS + 0, sr[0]);
       tmem_ld32(tS + 32, sr[1]);
@@ -387,7 +467,7 @@ __device__ void soften(const PagedArgs &a, const Division &d, Walk &walk,
         sl = 1.f;
       }
       const int base = j * a.tile_keys;
-      if (base + kTileRows > all_see || a.tile_keys < kTileRows) {
+      if (base + kTileRows > all_see) {
         const int lim = min(seen - base, a.tile_keys);
 #pragma unroll
         for (int c = 0; c < 128; ++c) s[c] = c < lim ? s[c] : -INFINITY;
@@ -409,7 +489,7 @@ __device__ void soften(const PagedArgs &a, const Division &d, Walk &walk,
       if (!(mt < INFINITY)) sum = NAN;
       l = m == -INFINITY && mt < INFINITY ? 0.f : fmaf(l, corr, sum);
       // P V of the tile before has completed: S was issued after it
-      if (j > it.t0 && __any_sync(0xffffffffu, rescale)) {
+      if (j > t0 && __any_sync(0xffffffffu, rescale)) {
 #pragma unroll
         for (int h = 0; h < D / 32; ++h) {
           uint32_t o[32];
@@ -428,18 +508,27 @@ __device__ void soften(const PagedArgs &a, const Division &d, Walk &walk,
       mbar_arrive(&bars[C::kPFull + t]);
     }
 
-    const bool any = end > it.t0;  // O_t holds something of this part
+    if (threadIdx.x == 0) FA_TRACE_CTA(3);
+    const bool whole = job->whole();
+    const Division d = ctrl->division;
+    // A split item's parts are joined by the last CTA to finish one. If all
+    // the others have by now, it need not write its own first.
+    uint32_t *counter = whole ? nullptr : a.counters + 2 * d.owner(job->at) + t;
+    const uint32_t mine = job->t1 - t0;
+    if (!whole && row == 0) {
+      const uint32_t had = atomicAdd(counter, 0u);
+      ctrl->join[t] = had + mine == static_cast<uint32_t>(job->tiles);
+      __threadfence();
+    }
+    const bool any = end > t0;  // O_t holds something of this part
     if (any) {
-      if (!mbar_wait(&bars[C::kODone + t], (done - 1) & 1)) {
-        ctrl->abort = 1;
-        return;
-      }
+      if (!mbar_wait(&bars[C::kODone + t], (done - 1) & 1)) return false;
       tc_fence_after();
     }
-    const size_t out_row =
-        static_cast<size_t>(it.seq.lo + token) * a.H + it.h * group + row - tok * group;
+    const size_t out_row = static_cast<size_t>(job->token + max(tok, 0)) * a.H +
+                           job->h * group + row % group;
     __half *dst = a.out + out_row * D;
-    if (it.whole()) {
+    if (whole) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
       for (int h = 0; h < D / 32; ++h) {
@@ -460,89 +549,131 @@ __device__ void soften(const PagedArgs &a, const Division &d, Walk &walk,
       continue;
     }
 
-    // ---- a part: kept, and joined with the others by the last to finish
-    auto slot = [&](int c, int t0) {
+    // ---- a part
+    auto slot = [&](int c, int first) {
       return a.partials +
-             ((2 * static_cast<size_t>(c) + slot_of(t0)) * 2 + t) * C::kSlotFloats;
+             ((2 * static_cast<size_t>(c) + slot_of(first)) * 2 + t) * C::kSlotFloats;
     };
-    float *mine = slot(blockIdx.x, it.t0);
+    if (!meet()) return false;
+    bool last = ctrl->join[t] != 0;
+    if (!last) {
+      float *p = slot(blockIdx.x, t0);
 #pragma unroll
-    for (int h = 0; h < D / 32; ++h) {
-      uint32_t o[32];
-      if (any && !idle) {
-        tmem_ld32(tO + 32 * h, o);
-        tmem_wait_ld();
-      }
-      if (real && l != 0.f) {
+      for (int h = 0; h < D / 32; ++h) {
+        uint32_t o[32];
+        if (any && !idle) {
+          tmem_ld32(tO + 32 * h, o);
+          tmem_wait_ld();
+        }
+        if (real && l != 0.f) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          *reinterpret_cast<uint4 *>(mine + ((8 * h + c) * kRows + row) * 4) =
-              make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
-      }
-    }
-    mine[D * kRows + row] = m;
-    mine[(D + 1) * kRows + row] = l;
-    __threadfence();
-    // the tile's 128 threads meet (bounded, like every wait here)
-    auto meet = [&]() {
-      mbar_arrive(&bars[C::kJoin + t]);
-      const bool ok = mbar_wait(&bars[C::kJoin + t], met & 1);
-      ++met;
-      if (!ok) ctrl->abort = 1;
-      return ok;
-    };
-    if (!meet()) return;
-    if (row == 0) {
-      uint32_t *counter = a.counters + 2 * d.owner(it.at) + t;
-      const uint32_t had = atomicAdd(counter, it.t1 - it.t0);
-      ctrl->join[t] = had + (it.t1 - it.t0) == static_cast<uint32_t>(it.tiles);
-      if (ctrl->join[t]) *counter = 0;
-      __threadfence();
-    }
-    if (!meet()) return;
-    if (!ctrl->join[t] || !real) continue;
-    const int c0 = d.owner(it.at), c1 = d.owner(it.at + it.cost - 1);
-    float M = -INFINITY;
-    for (int c = c0; c <= c1; ++c) {
-      int t0, t1;
-      tiles_of_cta(a, d, it, c, t0, t1);
-      if (t0 >= t1) continue;
-      const float *p = slot(c, t0);
-      if (__ldcg(p + (D + 1) * kRows + row) != 0.f)
-        M = fmaxf(M, __ldcg(p + D * kRows + row));
-    }
-    float L = 0.f;
-#pragma unroll
-    for (int h = 0; h < D / 32; ++h) {
-      float acc[32];
-#pragma unroll
-      for (int c = 0; c < 32; ++c) acc[c] = 0.f;
-      for (int c = c0; c <= c1; ++c) {
-        int t0, t1;
-        tiles_of_cta(a, d, it, c, t0, t1);
-        if (t0 >= t1) continue;
-        const float *p = slot(c, t0);
-        const float lc = __ldcg(p + (D + 1) * kRows + row);
-        if (lc == 0.f) continue;  // saw nothing
-        const float w = fast_exp2(__ldcg(p + D * kRows + row) - M);
-        if (h == 0) L = fmaf(lc, w, L);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float4 v = __ldcg(reinterpret_cast<const float4 *>(p) +
-                                  (8 * h + k) * kRows + row);
-          acc[4 * k] = fmaf(v.x, w, acc[4 * k]);
-          acc[4 * k + 1] = fmaf(v.y, w, acc[4 * k + 1]);
-          acc[4 * k + 2] = fmaf(v.z, w, acc[4 * k + 2]);
-          acc[4 * k + 3] = fmaf(v.w, w, acc[4 * k + 3]);
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<uint4 *>(p + ((8 * h + c) * kRows + row) * 4) =
+                make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
         }
       }
-      uint32_t o[32];
-#pragma unroll
-      for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(acc[c]);
-      store_dims<D, Dt>(dst + 32 * h, o, L == 0.f ? 0.f : 1.f / L);
+      p[D * kRows + row] = m;
+      p[(D + 1) * kRows + row] = l;
+      __threadfence();
+      if (threadIdx.x == 0) FA_TRACE_CTA(4);
+      if (!meet()) return false;
+      if (row == 0) {
+        const uint32_t had = atomicAdd(counter, mine);
+        ctrl->join[t] = had + mine == static_cast<uint32_t>(job->tiles);
+        __threadfence();
+      }
+      if (!meet()) return false;
+      last = ctrl->join[t] != 0;
     }
-    if (a.lse)
+    if (threadIdx.x == 0) FA_TRACE_CTA(5);
+    if (!last) continue;
+    if (row == 0) *counter = 0;
+    if (idle) continue;
+    Part it;
+    it.at = job->at;
+    it.cost = job->cost;
+    it.tiles = job->tiles;
+    const int c0 = d.owner(it.at), c1 = d.owner(it.at + it.cost - 1);
+    // a part's place, maximum and sum for this row (no place: our own)
+    auto part = [&](int c, const float *&p, float &mc, float &lc) {
+      int p0, p1;
+      tiles_of_cta(a, d, it, c, p0, p1);
+      p = nullptr;
+      mc = m;
+      lc = p0 < p1 ? l : 0.f;
+      if (p0 < p1 && c != static_cast<int>(blockIdx.x)) {
+        p = slot(c, p0);
+        mc = __ldcg(p + D * kRows + row);
+        lc = __ldcg(p + (D + 1) * kRows + row);
+      }
+    };
+    float M = -INFINITY, L = 0.f;
+    for (int c = c0; c <= c1; ++c) {
+      const float *p;
+      float mc, lc;
+      part(c, p, mc, lc);
+      if (lc != 0.f) M = fmaxf(M, mc);
+    }
+    for (int c = c0; c <= c1; ++c) {
+      const float *p;
+      float mc, lc;
+      part(c, p, mc, lc);
+      if (lc != 0.f) L = fmaf(lc, fast_exp2(mc - M), L);
+    }
+    constexpr int kDims = 64;  // of a row at a time
+#pragma unroll 1
+    for (int d0 = 0; d0 < D; d0 += kDims) {
+      float acc[kDims];
+#pragma unroll
+      for (int k = 0; k < kDims; ++k) acc[k] = 0.f;
+      for (int c = c0; c <= c1; ++c) {
+        const float *p;
+        float mc, lc;
+        part(c, p, mc, lc);
+        // a part that saw nothing has left no O
+        const float w = lc != 0.f ? fast_exp2(mc - M) : 0.f;
+        if (p) {
+          float4 x[kDims / 4];
+#pragma unroll
+          for (int k = 0; k < kDims / 4; ++k)
+            x[k] = __ldcg(reinterpret_cast<const float4 *>(p) + (d0 / 4 + k) * kRows + row);
+          if (w != 0.f && real) {
+#pragma unroll
+            for (int k = 0; k < kDims / 4; ++k) {
+              acc[4 * k] = fmaf(x[k].x, w, acc[4 * k]);
+              acc[4 * k + 1] = fmaf(x[k].y, w, acc[4 * k + 1]);
+              acc[4 * k + 2] = fmaf(x[k].z, w, acc[4 * k + 2]);
+              acc[4 * k + 3] = fmaf(x[k].w, w, acc[4 * k + 3]);
+            }
+          }
+        } else if (any && c == static_cast<int>(blockIdx.x)) {
+#pragma unroll
+          for (int h = 0; h < kDims / 32; ++h) {
+            uint32_t o[32];
+            tmem_ld32(tO + d0 + 32 * h, o);
+            tmem_wait_ld();
+            if (w != 0.f) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                acc[32 * h + k] = fmaf(__uint_as_float(o[k]), w, acc[32 * h + k]);
+            }
+          }
+        }
+      }
+      if (real) {
+#pragma unroll
+        for (int h = 0; h < kDims / 32; ++h) {
+          uint32_t o[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(acc[32 * h + c]);
+          store_dims<D, Dt>(dst + d0 + 32 * h, o, L == 0.f ? 0.f : 1.f / L);
+        }
+      }
+    }
+    if (real && a.lse)
       a.lse[out_row] = L == 0.f ? -INFINITY : 0.69314718055994531f * (M + log2f(L));
+    __syncwarp();
+    if (threadIdx.x == 0) FA_TRACE_CTA(6);
   }
 }
 
@@ -557,48 +688,57 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lane = threadIdx.x & 31;
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kBarOff);
   PlanSmem *ps = reinterpret_cast<PlanSmem *>(smem + C::kMiscOff);
-  Ctrl *ctrl = reinterpret_cast<Ctrl *>(smem + C::kMiscOff + sizeof(PlanSmem));
+  Ctrl *ctrl = reinterpret_cast<Ctrl *>(smem + C::kCtrlOff);
+  static_assert(sizeof(Ctrl) <= 512, "Ctrl has its place");
+  if (threadIdx.x == 0) FA_TRACE_CTA(0);
   if (smem_u32(smem) & 1023u) {
     if (threadIdx.x == 0) record_error(FA_ERR_SMEM_ALIGN);
     return;
   }
-  if (warp == kProducerWarp && lane == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&bars[C::kFull + s], 1);
-      mbar_init(&bars[C::kEmpty + s], 1);
-    }
-    mbar_init(&bars[C::kTail], 1);
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(&bars[C::kQFull + t], 1);
-      mbar_init(&bars[C::kQEmpty + t], 1);
-      mbar_init(&bars[C::kSFull + t], 1);
-      mbar_init(&bars[C::kPFull + t], 128);
-      mbar_init(&bars[C::kODone + t], 1);
-      mbar_init(&bars[C::kJoin + t], 128);
-    }
-    mbar_init(&bars[C::kDrain], 1);
-    fence_barrier_init();
-    prefetch_tensormap(&tm_q);
-    prefetch_tensormap(&tm_k);
-    prefetch_tensormap(&tm_v);
-    ctrl->abort = device_failed() ? 1u : 0u;
-  }
-  // Pages that do not fill a tile leave its last rows unwritten: V is zero
-  // there (and K's scores are masked).
-  if (a.tile_keys < kTileRows) {
-    const int chunks = (kTileRows - a.tile_keys) * 8;
-    for (int i = threadIdx.x; i < C::kStages * (D / 64) * chunks; i += kThreads) {
-      const int half = i / chunks, e = a.tile_keys * 8 + i % chunks;
-      *reinterpret_cast<uint4 *>(smem + C::kRingOff + half / (D / 64) * C::kStage +
-                                 C::kTile + half % (D / 64) * C::kHalf + 16 * e) =
-          make_uint4(0, 0, 0, 0);
-    }
-    fence_proxy_async_smem();
-  }
   Division d;
   Walk walk;
-  if (!plan<kThreads>(a, *ps, d, walk)) return;  // synchronises the CTA
-  if (ctrl->abort) return;
+  const bool work = plan<kThreads>(a, *ps, d, walk, [&] {
+    if (warp == kProducerWarp && lane == 0) {
+      for (int s = 0; s < C::kStages; ++s) {
+        mbar_init(&bars[C::kFull + s], 2);  // K, V
+        mbar_init(&bars[C::kEmpty + s], 1);
+      }
+      mbar_init(&bars[C::kTail], 1);
+      for (int t = 0; t < 2; ++t) {
+        mbar_init(&bars[C::kQFull + t], 1);
+        mbar_init(&bars[C::kQEmpty + t], 1);
+        mbar_init(&bars[C::kSFull + t], 1);
+        mbar_init(&bars[C::kPFull + t], 128);
+        mbar_init(&bars[C::kODone + t], 1);
+        mbar_init(&bars[C::kJoin + t], 128);
+      }
+      for (int p = 0; p < kParts; ++p) {
+        mbar_init(&bars[C::kPartFull + p], 1);
+        mbar_init(&bars[C::kPartEmpty + p], 11);  // warps that take parts
+      }
+      mbar_init(&bars[C::kDrain], 1);
+      fence_barrier_init();
+      prefetch_tensormap(&tm_q);
+      prefetch_tensormap(&tm_k);
+      prefetch_tensormap(&tm_v);
+      ctrl->abort = 0;
+    }
+    // Pages that do not fill a tile leave its last rows unwritten: V is zero
+    // there (and K's scores are masked).
+    if (a.tile_keys < kTileRows) {
+      const int chunks = (kTileRows - a.tile_keys) * 8;
+      for (int i = threadIdx.x; i < C::kStages * (D / 64) * chunks; i += kThreads) {
+        const int half = i / chunks, e = a.tile_keys * 8 + i % chunks;
+        *reinterpret_cast<uint4 *>(smem + C::kRingOff + half / (D / 64) * C::kStage +
+                                   C::kTile + half % (D / 64) * C::kHalf + 16 * e) =
+            make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+    }
+  });
+  if (!work) return;
+  if (threadIdx.x == 0) FA_TRACE_CTA(1);
+  if (threadIdx.x == 0) ctrl->division = d;
   if (warp == kMmaWarp) {
     tmem_alloc(&ctrl->tmem, 512);
     tmem_relinquish();
@@ -610,12 +750,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= kProducerWarp) {
     setmaxnreg_dec<kCtrlRegs>();
     if (warp == kProducerWarp)
-      produce<D>(a, walk, smem, bars, ctrl, &tm_q, &tm_k, &tm_v);
+      produce<D, false>(a, smem, bars, ctrl, &tm_q, &tm_k);
+    else if (warp == kProducerWarpV)
+      produce<D, true>(a, smem, bars, ctrl, &tm_q, &tm_v);
     else if (warp == kMmaWarp)
-      issue<D, Dt>(a, walk, smem, bars, ctrl);
+      issue<D, Dt>(a, smem, bars, ctrl);
+    else {
+      if (lane == 0) hand_out<D>(a, walk, bars, ctrl);
+      __syncwarp();
+    }
   } else {
     setmaxnreg_inc<kSoftmaxRegs>();
-    soften<D, Dt>(a, d, walk, bars, ctrl);
+    if (!soften<D, Dt>(a, bars, ctrl)) ctrl->abort = 1;
   }
   tc_fence_before();
   __syncthreads();

@@ -42,6 +42,14 @@ __host__ __device__ inline int tile_keys(int page_rows) {
   return page_rows < kTileRows ? kTileRows / page_rows * page_rows : kTileRows;
 }
 
+// a / b of non-negative numbers, which mostly fit 32 bits (a 64-bit division
+// takes four times as long).
+__host__ __device__ __forceinline__ long long divide(long long a, long long b) {
+  return static_cast<unsigned long long>(a | b) >> 32 == 0
+             ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b))
+             : a / b;
+}
+
 // One sequence of the step.
 struct Seq {
   int lo;          // first packed token
@@ -63,7 +71,7 @@ __host__ __device__ __forceinline__ long long cost_before(const PagedArgs &a,
                                                  const Seq &s, long long p) {
   if (!a.causal) return p * (a.item_cost + max(s.len, 0ll));
   const long long t = a.item_tokens, c = s.len - s.n;
-  const long long z = c < 0 ? min(p, -c / t) : 0;  // items that end before row 0
+  const long long z = c < 0 ? min(p, divide(-c, t)) : 0;  // items that end before row 0
   return p * a.item_cost + (p - z) * c + t * (p * (p + 1) - z * (z + 1)) / 2;
 }
 __host__ __device__ __forceinline__ int items_of(const PagedArgs &a, const Seq &s) {
@@ -87,14 +95,25 @@ struct Part {
   __host__ __device__ bool whole() const { return t0 == 0 && t1 == tiles; }
 };
 
-// The step's division, the same in every CTA.
+// The step's division, the same in every CTA: the first `extra` pieces are
+// one longer than the others.
 struct Division {
-  long long total;
+  long long each;
+  int extra;
   int ctas;  // CTAs with work
-  __host__ __device__ long long piece(long long c) const { return c * total / ctas; }
+  __host__ __device__ void set(long long total, int n) {
+    ctas = n;
+    each = divide(total, n);
+    extra = static_cast<int>(total - each * n);
+  }
+  __host__ __device__ long long piece(int c) const {
+    return c * each + (c < extra ? c : extra);
+  }
   // the CTA whose piece holds position u
   __host__ __device__ int owner(long long u) const {
-    return static_cast<int>(((u + 1) * ctas - 1) / total);
+    const long long longer = extra * (each + 1);
+    return static_cast<int>(u < longer ? divide(u, each + 1)
+                                       : extra + divide(u - longer, each));
   }
 };
 
@@ -110,9 +129,10 @@ __host__ __device__ __forceinline__ int rows_seen(const PagedArgs &a, const Seq 
 __host__ __device__ __forceinline__ int tile_at(const PagedArgs &a, int tiles,
                                        long long x) {
   const long long k = x - a.item_cost;
+  // k is at most an item's keys, so it fits 32 bits
   return k <= 0 ? 0
-                : static_cast<int>(
-                      min(static_cast<long long>(tiles), (k + a.tile_keys - 1) / a.tile_keys));
+                : min(tiles, static_cast<int>((static_cast<uint32_t>(k) +
+                                               a.tile_keys - 1) / a.tile_keys));
 }
 
 // Walks the parts of one CTA.
@@ -158,38 +178,46 @@ struct Walk {
 // The walk of the piece [u0, u1), which begins in sequence b, whose items
 // begin at position `at` of the step's cost.
 __host__ __device__ __forceinline__ void start(const PagedArgs &a, Walk &w,
-                                               int b, long long at) {
+                                               int b, const Seq &s,
+                                               long long at) {
   w.b = b;
-  w.s = read_seq(a, b);
-  const long long head = cost_of(a, w.s);
-  w.h = static_cast<int>((w.u0 - at) / head);
+  w.s = s;
+  const long long head = cost_of(a, s);
+  w.h = static_cast<int>(divide(w.u0 - at, head));
   const long long x = w.u0 - at - w.h * head;
-  int lo = 0, hi = items_of(a, w.s) - 1;  // the last item that starts by x
+  int lo = 0, hi = items_of(a, s) - 1;  // the last item that starts by x
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (cost_before(a, w.s, mid) <= x) lo = mid; else hi = mid - 1;
+    if (cost_before(a, s, mid) <= x) lo = mid; else hi = mid - 1;
   }
   w.p = lo;
-  w.at = at + w.h * head + cost_before(a, w.s, lo);
+  w.at = at + w.h * head + cost_before(a, s, lo);
 }
 
 struct PlanSmem {
   long long warp_sum[16];
-  long long at;
-  int b;
+  Walk walk;
+  int failed;
 };
 
 // Called by all kThreads threads of a CTA: the division of the step and this
-// CTA's walk. False if it has no work.
-template <int kThreads>
+// CTA's walk. False if it has no work. `prepare` runs in the shadow of the
+// lengths' loads and is seen by all threads afterwards.
+template <int kThreads, typename F>
 __device__ __forceinline__ bool plan(const PagedArgs &a, PlanSmem &sm,
-                                     Division &d, Walk &w) {
+                                     Division &d, Walk &w, F prepare) {
   static_assert(kThreads % 32 == 0 && kThreads <= 512, "one sum per warp");
   const int tid = threadIdx.x;
+  // thread i adds up sequences [b0, b1); mostly one
   const int each = (a.batch + kThreads - 1) / kThreads;
   const int b0 = min(tid * each, a.batch), b1 = min(b0 + each, a.batch);
-  long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += cost_of(a, read_seq(a, b));
+  Seq first{};
+  if (b0 < b1) first = read_seq(a, b0);
+  bool failed = false;
+  if (tid == kThreads - 1) failed = device_failed();
+  prepare();
+  long long mine = b0 < b1 ? cost_of(a, first) : 0;
+  for (int b = b0 + 1; b < b1; ++b) mine += cost_of(a, read_seq(a, b));
   mine *= a.H_kv;
   long long upto = mine;  // inclusive prefix within the warp
 #pragma unroll
@@ -198,6 +226,7 @@ __device__ __forceinline__ bool plan(const PagedArgs &a, PlanSmem &sm,
     if ((tid & 31) >= o) upto += v;
   }
   if ((tid & 31) == 31) sm.warp_sum[tid >> 5] = upto;
+  if (tid == kThreads - 1) sm.failed = failed;
   __syncthreads();
   long long total = 0, before = 0;
 #pragma unroll
@@ -206,26 +235,27 @@ __device__ __forceinline__ bool plan(const PagedArgs &a, PlanSmem &sm,
     total += sm.warp_sum[i];
   }
   before += upto - mine;
-  d.total = total;
-  d.ctas = static_cast<int>(
-      min(static_cast<long long>(gridDim.x), max(1ll, total / a.min_piece)));
-  const int c = blockIdx.x;
-  if (total == 0 || c >= d.ctas) return false;
+  const int grid = gridDim.x, c = blockIdx.x;
+  d.set(total, total >= static_cast<long long>(grid) * a.min_piece
+                   ? grid
+                   : max(1, static_cast<int>(divide(total, a.min_piece))));
+  if (total == 0 || c >= d.ctas || sm.failed) return false;
   w.u0 = d.piece(c);
   w.u1 = d.piece(c + 1);
-  if (mine > 0 && before <= w.u0 && w.u0 < before + mine) {
+  if (before <= w.u0 && w.u0 < before + mine) {  // one thread
     int b = b0;
     long long at = before;
-    for (;; ++b) {
-      const long long here = cost_of(a, read_seq(a, b)) * a.H_kv;
+    for (;;) {
+      const long long here = cost_of(a, first) * a.H_kv;
       if (w.u0 < at + here) break;
       at += here;
+      first = read_seq(a, ++b);
     }
-    sm.b = b;
-    sm.at = at;
+    start(a, w, b, first, at);
+    sm.walk = w;
   }
   __syncthreads();
-  start(a, w, sm.b, sm.at);
+  w = sm.walk;
   return true;
 }
 
