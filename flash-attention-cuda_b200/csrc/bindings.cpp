@@ -645,10 +645,8 @@ void paged_call(const at::Tensor &rows, const at::Tensor &starts,
   TORCH_CHECK(k_pages.size(0) > 0 && k_pages.size(1) > 0,
               "k_pages must hold at least one page and head, got ",
               k_pages.sizes());
-  TORCH_CHECK(page_rows > 0 && page_rows % 8 == 0 &&
-                  (page_rows <= 128 || page_rows % 128 == 0),
-              "a page must have a multiple of 8 rows, and above 128 a "
-              "multiple of 128, got ", page_rows);
+  TORCH_CHECK(page_rows > 0 && page_rows % 8 == 0,
+              "a page must have a multiple of 8 rows, got ", page_rows);
   check_int32(starts, "starts", rows);
   check_int32(seq_lens, "seq_lens", rows);
   check_int32(page_table, "page_table", rows);

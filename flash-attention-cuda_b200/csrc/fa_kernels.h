@@ -171,9 +171,9 @@ struct PagedArgs {
   int batch, tokens, H, H_kv, D, table_width, page_rows, num_pages;
   float scale_log2;
   int causal;
-  // set by the launch: keys of a key tile, new tokens of an item, and the
+  // set by the launch: rows of a TMA box, new tokens of an item, and the
   // division of the work (paged_sm100.cuh)
-  int tile_keys, item_tokens, item_cost, min_piece;
+  int box_rows, item_tokens, item_cost, min_piece, min_part;
   float *partials;
   uint32_t *counters;
 };

@@ -25,7 +25,7 @@ cudaError_t launch(const PagedArgs &a, int form, const CUtensorMap &tm_q,
                    cudaStream_t stream) {
   if (form == kPagedFew)
     few::attend_few_kernel<D, Dt>
-        <<<min(sms, few::kMaxGrid), few::kThreads, few::Cfg<D>::kSmemBytes, stream>>>(a, tm_k, tm_v);
+        <<<min(sms, few::kMaxGrid), few::Cfg<D>::kThreads, few::Cfg<D>::kSmemBytes, stream>>>(a, tm_k, tm_v);
   else
     many::attend_many_kernel<D, Dt>
         <<<sms, many::kThreads, many::Cfg<D>::kSmemBytes, stream>>>(a, tm_q, tm_k,
@@ -70,17 +70,20 @@ int attend_paged_form(const PagedArgs &a) {
 
 void attend_paged_plan(PagedArgs &a, int form) {
   const int group = a.H / a.H_kv;
-  a.tile_keys = paged::tile_keys(a.page_rows);
+  a.box_rows = paged::box_rows(a.page_rows);
+  a.min_part = 1;
   if (form == kPagedFew) {
     a.item_tokens = paged::few::kRows / group;
-    a.item_cost = 128;
-    a.min_piece = 256;
+    a.item_cost = 384;
+    a.min_piece = 640;
   } else {
     a.item_tokens = 2 * (paged::many::kRows / group);
     a.item_cost = 256;
     a.min_piece = 512;
+    a.min_part = 2;
   }
 #ifdef FA_TUNE
+  if (getenv("FA_PART")) a.min_part = atoi(getenv("FA_PART"));
   if (getenv("FA_COST")) a.item_cost = atoi(getenv("FA_COST"));
   if (getenv("FA_PIECE")) a.min_piece = atoi(getenv("FA_PIECE"));
 #endif

@@ -40,8 +40,7 @@ int check_cache(const fa_paged_cache *c) {
   if (c->num_pages <= 0 || c->kv_heads <= 0 || c->page_rows <= 0 ||
       c->table_width <= 0 || c->table_stride < 0)
     return FA_EINVAL;
-  if (c->page_rows % 8 != 0 || (c->page_rows > 128 && c->page_rows % 128 != 0))
-    return FA_EINVAL;
+  if (c->page_rows % 8 != 0) return FA_EINVAL;
   const int sizes[3] = {c->num_pages, c->kv_heads, c->page_rows};
   const int64_t ks[3] = {c->k_page_stride, c->k_head_stride, c->k_row_stride};
   const int64_t vs[3] = {c->v_page_stride, c->v_head_stride, c->v_row_stride};
@@ -316,13 +315,12 @@ int fa_attend_paged(const void *q, const int64_t q_strides[2], void *o,
   const int form = attend_paged_form(a);
   attend_paged_plan(a, form);
   const int group = H / c.kv_heads;
-  const int box = c.page_rows < 128 ? c.page_rows : 128;
   const int kv_sizes[4] = {c.head_dim, c.page_rows, c.kv_heads, c.num_pages};
   const int64_t k_str[3] = {c.k_row_stride, c.k_head_stride, c.k_page_stride};
   const int64_t v_str[3] = {c.v_row_stride, c.v_head_stride, c.v_page_stride};
   CUtensorMap tq{}, tk, tv;
-  if (make_map(&tk, c.k_pages, dtype, kv_sizes, k_str, box, 1) != FA_OK ||
-      make_map(&tv, c.v_pages, dtype, kv_sizes, v_str, box, 1) != FA_OK)
+  if (make_map(&tk, c.k_pages, dtype, kv_sizes, k_str, a.box_rows, 1) != FA_OK ||
+      make_map(&tv, c.v_pages, dtype, kv_sizes, v_str, a.box_rows, 1) != FA_OK)
     return FA_EINVAL;
   if (form == kPagedMany) {
     // (dims, heads of a group, groups, tokens): a box is a tile's rows in

@@ -31,14 +31,17 @@ namespace few {
 
 constexpr int kRows = 16;  // query rows of an item
 constexpr int kWarps = 8;  // consumers
-constexpr int kProducers = 2;  // one warp for K, one for V
-constexpr int kThreads = 32 * (kWarps + kProducers);
 constexpr int kMaxGrid = 160;  // CTAs (statistics of a join in shared memory)
 constexpr float kNegBig = -1e30f;  // the maximum of no scores yet
 
 template <int D>
 struct Cfg {
-  static constexpr uint32_t kHalf = kTileRows * 128;   // 64 dims of a tile
+  // Producer warps: one for every 64 dims of K and of V. A warp issues a box
+  // in 50 ns, and small pages make many: with 8-row pages of 128 dims one
+  // warp took 324 us, two 229 where 64-row pages take 161.
+  static constexpr int kProducers = 2 * (D / 64);
+  static constexpr int kThreads = 32 * (kWarps + kProducers);
+  static constexpr uint32_t kHalf = kTileKeys * 128;   // 64 dims of a tile
   static constexpr uint32_t kTile = D / 64 * kHalf;    // K or V
   static constexpr uint32_t kStage = 2 * kTile;
   static constexpr int kStages = 6 * 64 / D;           // 192 KiB
@@ -245,9 +248,9 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
         break;
       }
       if (threadIdx.x == 0 && pos == 0) FA_TRACE_CTA(2);
-      const int base = i * a.tile_keys;
+      const int base = i * kTileKeys;
       // rows of this warp that the tile holds
-      const int here = min(it.keys - base, a.tile_keys) - key0;
+      const int here = min(it.keys - base, kTileKeys) - key0;
       if (here > 0) {  // warp-uniform
         const uint32_t kb = smem_u32(smem + slot * C::kStage);
         const uint32_t vb = kb + C::kTile;
@@ -411,7 +414,7 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
 }
 
 template <int D, typename Dt>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     attend_few_kernel(const PagedArgs a, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v) {
   using C = Cfg<D>;
@@ -431,10 +434,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   Division d;
   Walk walk;
-  const bool work = plan<kThreads>(a, *ps, d, walk, [&] {
+  const bool work = plan<C::kThreads>(a, *ps, d, walk, [&] {
     if (warp == kWarps && lane == 0) {
       for (int s = 0; s < C::kStages; ++s) {
-        mbar_init(&full[s], kProducers);
+        mbar_init(&full[s], C::kProducers);
         mbar_init(&empty[s], kWarps);
       }
       fence_barrier_init();
@@ -449,35 +452,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     consume<D, Dt>(a, d, walk, smem, full, empty);
     return;
   }
-  // ---- producers, one of K and one of V (small pages make many boxes, and
-  // a warp issues one in 50 ns): lane j loads page j of the tile
-  const bool is_v = warp > kWarps;
-  const CUtensorMap *map = is_v ? &tm_v : &tm_k;
-  const int box = min(a.page_rows, kTileRows);
+  // ---- producers: lane j loads box j of the tile
+  const int part = warp - kWarps;  // K's halves, then V's
+  const CUtensorMap *map = part < D / 64 ? &tm_k : &tm_v;
+  const int dim = 64 * (part % (D / 64));
+  const uint32_t box = a.box_rows * 128;
+  uint8_t *to = smem + part * C::kHalf + lane * box;
   int pos = 0;
   bool ok = true;
   Part it;
+  Boxes boxes;
   while (ok && walk.next(a, it)) {
-    int page = it.t0 < it.t1 ? tile_page(a, it.b, it.keys, it.t0, lane) : -1;
+    if (it.t0 < it.t1) boxes.open(a, it.b, it.keys, it.t0);
     for (int i = it.t0; i < it.t1; ++i, ++pos) {
-      const int next = i + 1 < it.t1 ? tile_page(a, it.b, it.keys, i + 1, lane) : -1;
+      int row;
+      const int page = boxes.take(a, row);
       const int slot = pos % C::kStages, use = pos / C::kStages;
       if (use > 0 && !mbar_wait(&empty[slot], (use - 1) & 1)) {
         ok = false;
         break;
       }
-      const uint32_t pages = __ballot_sync(0xffffffffu, page >= 0);
-      if (lane == 0)
-        mbar_arrive_expect_tx(&full[slot], __popc(pages) * box * 128 * (D / 64));
+      const uint32_t loads = __ballot_sync(0xffffffffu, page >= 0);
+      if (lane == 0) mbar_arrive_expect_tx(&full[slot], __popc(loads) * box);
       __syncwarp();
-      if (page >= 0) {
-        const int row = a.page_rows < kTileRows ? 0 : i * a.tile_keys % a.page_rows;
-        uint8_t *to = smem + slot * C::kStage + (is_v ? C::kTile : 0) + lane * box * 128;
-#pragma unroll
-        for (int h = 0; h < D / 64; ++h)
-          tma_load_4d(to + h * C::kHalf, map, &full[slot], 64 * h, row, it.h, page);
-      }
-      page = next;
+      if (page >= 0)
+        tma_load_4d(to + slot * C::kStage, map, &full[slot], dim, row, it.h, page);
     }
   }
   // No copy may still be landing when the CTA exits: the consumers wait for

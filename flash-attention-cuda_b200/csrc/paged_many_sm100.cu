@@ -48,8 +48,8 @@ constexpr int kMmaWarp = 9;
 constexpr int kProducerWarpV = 10;
 constexpr int kWalkWarp = 11;
 constexpr int kParts = 4;  // parts handed out ahead
-constexpr int kCtrlRegs = 24;
-constexpr int kSoftmaxRegs = 240;
+constexpr int kCtrlRegs = 40;
+constexpr int kSoftmaxRegs = 232;
 static_assert(128 * kCtrlRegs + 256 * kSoftmaxRegs <= kThreads * 168,
               "register split exceeds the launch allocation");
 // O is rescaled only when a row's maximum has grown by more than this (in
@@ -58,7 +58,7 @@ constexpr float kRescaleThreshold = 8.0f;
 
 template <int D>
 struct Cfg {
-  static constexpr uint32_t kHalf = kTileRows * 128;  // 64 dims of 128 rows
+  static constexpr uint32_t kHalf = kTileKeys * 128;  // 64 dims of 128 rows
   static constexpr uint32_t kTile = D / 64 * kHalf;   // Q_t, K or V
   static constexpr uint32_t kStage = 2 * kTile;
   static constexpr int kStages = D == 128 ? 2 : 5;
@@ -88,7 +88,7 @@ struct Cfg {
 };
 
 template <typename Dt>
-constexpr uint32_t kIdescS = idesc_f16_f32(kRows, kTileRows, false, Dt::kFmt);
+constexpr uint32_t kIdescS = idesc_f16_f32(kRows, kTileKeys, false, Dt::kFmt);
 template <int D, typename Dt>
 constexpr uint32_t kIdescPV = idesc_f16_f32(kRows, D, true, Dt::kFmt);
 
@@ -107,7 +107,7 @@ template <int D, typename Dt>
 __device__ __forceinline__ void issue_pv(uint32_t d, uint32_t p, uint64_t v,
                                          bool accumulate) {
 #pragma unroll
-  for (int kk = 0; kk < kTileRows / 16; ++kk)
+  for (int kk = 0; kk < kTileKeys / 16; ++kk)
     mma_f16_ts(d, p + 8 * kk, v + 128 * kk, kIdescPV<D, Dt>,
                accumulate || kk > 0 ? 1u : 0u);
 }
@@ -190,7 +190,7 @@ __device__ void hand_out(const PagedArgs &a, Walk &walk, uint64_t *bars, Ctrl *c
       for (int t = 0; t < 2; ++t) {
         const int last = min(j.n, (t + 1) * tile_tokens(a)) - 1;
         const int end = last < t * tile_tokens(a)
-                            ? 0 : (job_seen(a, j, last) + a.tile_keys - 1) / a.tile_keys;
+                            ? 0 : tiles_of(job_seen(a, j, last));
         j.end[t] = max(it.t0, min(it.t1, end));
       }
     }
@@ -204,7 +204,7 @@ __device__ void produce(const PagedArgs &a, uint8_t *smem, uint64_t *bars,
                         Ctrl *ctrl, const CUtensorMap *tm_q, const CUtensorMap *tm) {
   using C = Cfg<D>;
   const int lane = threadIdx.x & 31;
-  const int box = min(a.page_rows, kTileRows);
+  const uint32_t box = a.box_rows * 128;
   int pos = 0, q_used[2] = {0, 0};
   uint32_t tail_phase = 0;
   bool ok = true;
@@ -215,7 +215,8 @@ __device__ void produce(const PagedArgs &a, uint8_t *smem, uint64_t *bars,
     const int token = job->token;
     const bool has[2] = {job->end[0] > t0, job->end[1] > t0};
     release<D>(bars, n);
-    int page = t0 < t1 ? tile_page(a, b, keys, t0, lane) : -1;
+    Boxes boxes;
+    if (t0 < t1) boxes.open(a, b, keys, t0);
     for (int t = 0; !kV && ok && t < 2; ++t) {
       if (!has[t]) continue;
       if (q_used[t] > 0 && !mbar_wait(&bars[C::kQEmpty + t], (q_used[t] - 1) & 1)) {
@@ -232,7 +233,8 @@ __device__ void produce(const PagedArgs &a, uint8_t *smem, uint64_t *bars,
       }
     }
     for (int i = t0; ok && i < t1; ++i, ++pos) {
-      const int next = i + 1 < t1 ? tile_page(a, b, keys, i + 1, lane) : -1;
+      int row;
+      const int page = boxes.take(a, row);
       const int slot = pos % C::kStages, use = pos / C::kStages;
       if (ctrl->abort ||
           (use > 0 && !mbar_wait(&bars[C::kEmpty + slot], (use - 1) & 1))) {
@@ -243,33 +245,29 @@ __device__ void produce(const PagedArgs &a, uint8_t *smem, uint64_t *bars,
       // of its own: the rows there may hold anything, NaN included, and are
       // cleared before the tile is handed on (P is zero there, and zero times
       // NaN is not).
-      const int valid = keys - i * a.tile_keys;
-      const bool tail = kV && valid < a.tile_keys;
+      const int valid = keys - i * kTileKeys;
+      const bool tail = kV && valid < kTileKeys;
       uint64_t *bar = &bars[tail ? C::kTail : C::kFull + slot];
-      const uint32_t pages = __ballot_sync(0xffffffffu, page >= 0);
-      if (lane == 0)
-        mbar_arrive_expect_tx(bar, __popc(pages) * box * 128 * (D / 64));
+      const uint32_t loads = __ballot_sync(0xffffffffu, page >= 0);
+      if (lane == 0) mbar_arrive_expect_tx(bar, __popc(loads) * box * (D / 64));
       __syncwarp();
       uint8_t *tile = smem + C::kRingOff + slot * C::kStage + (kV ? C::kTile : 0);
       if (page >= 0) {
-        const int row = a.page_rows < kTileRows ? 0 : i * a.tile_keys % a.page_rows;
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(tile + lane * box * 128 + c * C::kHalf, tm, bar, 64 * c, row, h,
-                      page);
+          tma_load_4d(tile + lane * box + c * C::kHalf, tm, bar, 64 * c, row, h, page);
       }
       if (tail) {
         ok = mbar_wait(bar, tail_phase);
         tail_phase ^= 1;
         for (int c = 0; c < D / 64; ++c)
-          for (int e = valid * 8 + lane; e < a.tile_keys * 8; e += 32)
+          for (int e = valid * 8 + lane; e < kTileKeys * 8; e += 32)
             *reinterpret_cast<uint4 *>(tile + c * C::kHalf + 16 * e) =
                 make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[C::kFull + slot]);
       }
-      page = next;
     }
   }
   if (!ok || ctrl->abort) {
@@ -439,8 +437,7 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
     // a warp without a row only keeps the tile's barriers going
     const bool idle = !__any_sync(0xffffffffu, real);
     // keys that every row of the tile sees
-    const int all_see =
-        a.tile_keys < kTileRows ? -1 : job_seen(a, *job, t * tile_tokens(a));
+    const int all_see = job_seen(a, *job, t * tile_tokens(a));
     float m = -INFINITY, l = 0.f;
 
     for (int j = t0; j < end; ++j, ++done) {
@@ -466,9 +463,9 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
         for (int c = 0; c < 128; ++c) s[c] *= a.scale_log2;
         sl = 1.f;
       }
-      const int base = j * a.tile_keys;
-      if (base + kTileRows > all_see) {
-        const int lim = min(seen - base, a.tile_keys);
+      const int base = j * kTileKeys;
+      if (base + kTileKeys > all_see) {
+        const int lim = seen - base;
 #pragma unroll
         for (int c = 0; c < 128; ++c) s[c] = c < lim ? s[c] : -INFINITY;
       }
@@ -515,11 +512,8 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
     // the others have by now, it need not write its own first.
     uint32_t *counter = whole ? nullptr : a.counters + 2 * d.owner(job->at) + t;
     const uint32_t mine = job->t1 - t0;
-    if (!whole && row == 0) {
-      const uint32_t had = atomicAdd(counter, 0u);
-      ctrl->join[t] = had + mine == static_cast<uint32_t>(job->tiles);
-      __threadfence();
-    }
+    uint32_t arrived = 0;
+    if (!whole && row == 0) arrived = __ldcg(counter);
     const bool any = end > t0;  // O_t holds something of this part
     if (any) {
       if (!mbar_wait(&bars[C::kODone + t], (done - 1) & 1)) return false;
@@ -550,6 +544,10 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
     }
 
     // ---- a part
+    if (row == 0) {
+      ctrl->join[t] = arrived + mine == static_cast<uint32_t>(job->tiles);
+      __threadfence();
+    }
     auto slot = [&](int c, int first) {
       return a.partials +
              ((2 * static_cast<size_t>(c) + slot_of(first)) * 2 + t) * C::kSlotFloats;
@@ -594,71 +592,55 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
     it.cost = job->cost;
     it.tiles = job->tiles;
     const int c0 = d.owner(it.at), c1 = d.owner(it.at + it.cost - 1);
-    // a part's place, maximum and sum for this row (no place: our own)
-    auto part = [&](int c, const float *&p, float &mc, float &lc) {
-      int p0, p1;
-      tiles_of_cta(a, d, it, c, p0, p1);
-      p = nullptr;
-      mc = m;
-      lc = p0 < p1 ? l : 0.f;
-      if (p0 < p1 && c != static_cast<int>(blockIdx.x)) {
-        p = slot(c, p0);
-        mc = __ldcg(p + D * kRows + row);
-        lc = __ldcg(p + (D + 1) * kRows + row);
-      }
-    };
-    float M = -INFINITY, L = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      const float *p;
-      float mc, lc;
-      part(c, p, mc, lc);
-      if (lc != 0.f) M = fmaxf(M, mc);
-    }
-    for (int c = c0; c <= c1; ++c) {
-      const float *p;
-      float mc, lc;
-      part(c, p, mc, lc);
-      if (lc != 0.f) L = fmaf(lc, fast_exp2(mc - M), L);
-    }
     constexpr int kDims = 64;  // of a row at a time
 #pragma unroll 1
     for (int d0 = 0; d0 < D; d0 += kDims) {
+      float M = -INFINITY, L = 0.f;
       float acc[kDims];
 #pragma unroll
       for (int k = 0; k < kDims; ++k) acc[k] = 0.f;
       for (int c = c0; c <= c1; ++c) {
-        const float *p;
-        float mc, lc;
-        part(c, p, mc, lc);
-        // a part that saw nothing has left no O
-        const float w = lc != 0.f ? fast_exp2(mc - M) : 0.f;
-        if (p) {
+        int p0, p1;
+        tiles_of_cta(a, d, it, c, p0, p1);
+        if (p0 >= p1) continue;
+        const bool own = c == static_cast<int>(blockIdx.x);
+        const float *p = slot(c, p0);
+        const float mc = own ? m : __ldcg(p + D * kRows + row);
+        const float lc = own ? l : __ldcg(p + (D + 1) * kRows + row);
+        const bool some = lc != 0.f && real;  // else it left no O
+        const float mn = some ? fmaxf(M, mc) : M;
+        const float s0 = some ? fast_exp2(M - mn) : 1.f;
+        const float s1 = some ? fast_exp2(mc - mn) : 0.f;
+        M = mn;
+        if (some) L = L * s0 + lc * s1;
+        if (!own) {
           float4 x[kDims / 4];
 #pragma unroll
           for (int k = 0; k < kDims / 4; ++k)
             x[k] = __ldcg(reinterpret_cast<const float4 *>(p) + (d0 / 4 + k) * kRows + row);
-          if (w != 0.f && real) {
+          if (some) {
 #pragma unroll
             for (int k = 0; k < kDims / 4; ++k) {
-              acc[4 * k] = fmaf(x[k].x, w, acc[4 * k]);
-              acc[4 * k + 1] = fmaf(x[k].y, w, acc[4 * k + 1]);
-              acc[4 * k + 2] = fmaf(x[k].z, w, acc[4 * k + 2]);
-              acc[4 * k + 3] = fmaf(x[k].w, w, acc[4 * k + 3]);
+              acc[4 * k] = fmaf(x[k].x, s1, acc[4 * k] * s0);
+              acc[4 * k + 1] = fmaf(x[k].y, s1, acc[4 * k + 1] * s0);
+              acc[4 * k + 2] = fmaf(x[k].z, s1, acc[4 * k + 2] * s0);
+              acc[4 * k + 3] = fmaf(x[k].w, s1, acc[4 * k + 3] * s0);
             }
           }
-        } else if (any && c == static_cast<int>(blockIdx.x)) {
+        } else if (any) {
 #pragma unroll
           for (int h = 0; h < kDims / 32; ++h) {
             uint32_t o[32];
             tmem_ld32(tO + d0 + 32 * h, o);
             tmem_wait_ld();
-            if (w != 0.f) {
+            if (some) {
 #pragma unroll
               for (int k = 0; k < 32; ++k)
-                acc[32 * h + k] = fmaf(__uint_as_float(o[k]), w, acc[32 * h + k]);
+                acc[32 * h + k] = fmaf(__uint_as_float(o[k]), s1, acc[32 * h + k] * s0);
             }
           }
         }
+        __syncwarp();
       }
       if (real) {
 #pragma unroll
@@ -668,10 +650,10 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
           for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(acc[32 * h + c]);
           store_dims<D, Dt>(dst + d0 + 32 * h, o, L == 0.f ? 0.f : 1.f / L);
         }
+        if (a.lse && d0 == 0)
+          a.lse[out_row] = L == 0.f ? -INFINITY : 0.69314718055994531f * (M + log2f(L));
       }
     }
-    if (real && a.lse)
-      a.lse[out_row] = L == 0.f ? -INFINITY : 0.69314718055994531f * (M + log2f(L));
     __syncwarp();
     if (threadIdx.x == 0) FA_TRACE_CTA(6);
   }
@@ -722,18 +704,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       prefetch_tensormap(&tm_k);
       prefetch_tensormap(&tm_v);
       ctrl->abort = 0;
-    }
-    // Pages that do not fill a tile leave its last rows unwritten: V is zero
-    // there (and K's scores are masked).
-    if (a.tile_keys < kTileRows) {
-      const int chunks = (kTileRows - a.tile_keys) * 8;
-      for (int i = threadIdx.x; i < C::kStages * (D / 64) * chunks; i += kThreads) {
-        const int half = i / chunks, e = a.tile_keys * 8 + i % chunks;
-        *reinterpret_cast<uint4 *>(smem + C::kRingOff + half / (D / 64) * C::kStage +
-                                   C::kTile + half % (D / 64) * C::kHalf + 16 * e) =
-            make_uint4(0, 0, 0, 0);
-      }
-      fence_proxy_async_smem();
     }
   });
   if (!work) return;

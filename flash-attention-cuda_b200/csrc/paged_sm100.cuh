@@ -35,11 +35,17 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map,
       : "memory");
 }
 
-constexpr int kTileRows = 128;  // key rows a tile has room for
+constexpr int kTileKeys = 128;
 
-// Keys of a tile: the whole pages that fit, or 128 rows of a larger page.
-__host__ __device__ inline int tile_keys(int page_rows) {
-  return page_rows < kTileRows ? kTileRows / page_rows * page_rows : kTileRows;
+// Rows of a TMA box: pages and tiles are both cut into whole boxes.
+__host__ __device__ inline int box_rows(int page_rows) {
+  int a = kTileKeys, b = page_rows;
+  while (b) {
+    const int r = a % b;
+    a = b;
+    b = r;
+  }
+  return a;
 }
 
 // a / b of non-negative numbers, which mostly fit 32 bits (a 64-bit division
@@ -125,14 +131,20 @@ __host__ __device__ __forceinline__ int rows_seen(const PagedArgs &a, const Seq 
   return static_cast<int>(max(0ll, min(min(r, s.len), cap)));
 }
 
-// The first tile that a position inside an item leaves to its right.
+__host__ __device__ __forceinline__ int tiles_of(int keys) {
+  return static_cast<int>((static_cast<uint32_t>(keys) + kTileKeys - 1) / kTileKeys);
+}
+
+// The first tile that a position inside an item leaves to its right. Parts of
+// less than a.min_part tiles cost more than the balance they bring: such a
+// position moves to the item's start or end.
 __host__ __device__ __forceinline__ int tile_at(const PagedArgs &a, int tiles,
-                                       long long x) {
+                                                long long x) {
   const long long k = x - a.item_cost;
+  if (k <= 0) return 0;
   // k is at most an item's keys, so it fits 32 bits
-  return k <= 0 ? 0
-                : min(tiles, static_cast<int>((static_cast<uint32_t>(k) +
-                                               a.tile_keys - 1) / a.tile_keys));
+  const int t = static_cast<int>((static_cast<uint32_t>(k) + kTileKeys - 1) / kTileKeys);
+  return t < a.min_part ? 0 : t > tiles - a.min_part ? tiles : t;
 }
 
 // Walks the parts of one CTA.
@@ -163,7 +175,7 @@ struct Walk {
       out.at = at;
       out.cost = a.item_cost + max(0ll, a.causal ? c + last + 1 : s.len);
       out.keys = rows_seen(a, s, s.n - 1);
-      out.tiles = (rows_seen(a, s, last) + a.tile_keys - 1) / a.tile_keys;
+      out.tiles = tiles_of(rows_seen(a, s, last));
       out.t0 = at >= u0 ? 0 : tile_at(a, out.tiles, u0 - at);
       out.t1 = at + out.cost <= u1 ? out.tiles : tile_at(a, out.tiles, u1 - at);
       const bool mine = out.tiles == 0 ? at >= u0 : out.t0 < out.t1;
@@ -272,25 +284,55 @@ __host__ __device__ __forceinline__ void tiles_of_cta(const PagedArgs &a,
 // not begin is the first of its piece, one that it does not end the last.
 __host__ __device__ __forceinline__ int slot_of(int t0) { return t0 > 0 ? 0 : 1; }
 
-// A page table entry for the tensor maps: one that is no page reads as the
-// page after the last, which TMA fills with zeros.
-__device__ __forceinline__ int page_entry(const PagedArgs &a, int b, int i) {
-  const int page = a.page_table[b * a.table_stride + i];
-  if (page >= 0 && page < a.num_pages) return page;
-  record_error(FA_ERR_PAGE);
-  return a.num_pages;
-}
+// The boxes of a part's key tiles, for a producer warp: lane j has box j of
+// a tile, the next tile's page table entries under way while it loads one.
+// (Kept lean: in the many-row kernel every instruction here takes an issue
+// slot from a softmax warp.)
+struct Boxes {
+  const int32_t *table;
+  int step_page, step_row;  // a tile's rows in whole pages and rows
+  int left;                 // rows of the sequence from this lane's box on
+  int index, row;           // its page table index and row there
+  int next, next_row;       // the coming tile's page (-1: none) and row
 
-// The page that lane `lane` of the producer warp loads for key tile i of a
-// sequence of `keys` rows, and the tile's first row in it; -1: none.
-__device__ __forceinline__ int tile_page(const PagedArgs &a, int b, int keys,
-                                         int i, int lane) {
-  const int row = i * a.tile_keys + (a.page_rows < kTileRows ? lane * a.page_rows : 0);
-  const bool has = a.page_rows < kTileRows
-                       ? lane < a.tile_keys / a.page_rows && row < keys
-                       : lane == 0;
-  return has ? page_entry(a, b, row / a.page_rows) : -1;
-}
+  __device__ __forceinline__ void look(const PagedArgs &a) {
+    next = left > 0 ? a.num_pages : -1;  // past the pool: TMA writes zeros
+    next_row = row;
+    if (left > 0) {
+      const int page = table[index];
+      if (page >= 0 && page < a.num_pages)
+        next = page;
+      else
+        record_error(FA_ERR_PAGE);
+    }
+    left -= kTileKeys;
+    index += step_page;
+    row += step_row;
+    if (row >= a.page_rows) {
+      row -= a.page_rows;
+      ++index;
+    }
+  }
+  // tiles from t0 on of sequence b, which has `keys` rows
+  __device__ __forceinline__ void open(const PagedArgs &a, int b, int keys, int t0) {
+    const int lane = threadIdx.x & 31;
+    const int first = t0 * kTileKeys + lane * a.box_rows;
+    left = lane * a.box_rows < kTileKeys ? keys - first : 0;
+    table = a.page_table + b * a.table_stride;
+    index = first / a.page_rows;
+    row = first - index * a.page_rows;
+    step_page = kTileKeys / a.page_rows;
+    step_row = kTileKeys - step_page * a.page_rows;
+    look(a);
+  }
+  // this lane's page and row of the tile, and on to the next one
+  __device__ __forceinline__ int take(const PagedArgs &a, int &at_row) {
+    const int page = next;
+    at_row = next_row;
+    look(a);
+    return page;
+  }
+};
 
 }  // namespace paged
 }  // namespace fa

@@ -477,8 +477,8 @@ int fa_rope(const void *q, const int64_t q_strides[3], void *q_out,
  * (page, h, row, d) of a pool lies at page * page_stride + h * head_stride +
  * row * row_stride + d (elements; strides are multiples of 8 and the pools
  * 16-byte aligned, so both (pages, heads, rows, head_dim) and (pages, rows,
- * heads, head_dim) pools serve). page_rows is a multiple of 8, and from 128
- * rows on a multiple of 128. A sequence holds at most table_width *
+ * heads, head_dim) pools serve). page_rows is a multiple of 8 (a multiple or
+ * divisor of 128 is read fastest). A sequence holds at most table_width *
  * page_rows rows. head_dim is 64 or 128. Table entries past a sequence's
  * rows are never read; one that is needed and is no page of the pool is
  * neither read nor written through: it sets FA_ERR_PAGE in the device error

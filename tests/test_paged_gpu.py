@@ -45,7 +45,7 @@ def test_attention_matches_the_definition(dtype, d, h, h_kv, news, lens):
 
 
 @pytest.mark.parametrize("token_major", [False, True])
-@pytest.mark.parametrize("page", [8, 16, 24, 56, 64, 96, 128, 256])
+@pytest.mark.parametrize("page", [8, 16, 24, 56, 64, 96, 128, 200, 256])
 @pytest.mark.parametrize("news,lens", [([1, 1, 1], [255, 256, 1000]),
                                        ([70, 129, 1], [70, 600, 385])])
 def test_page_sizes_and_layouts(token_major, page, news, lens):
