@@ -48,14 +48,16 @@ struct Cfg {
   // The warps' states at the end of a part: O, 16 KiB at a time, then (m, l)
   static constexpr uint32_t kRedOff = kStages * kStage;
   static constexpr uint32_t kRedBytes = 16384;
+  static constexpr uint32_t kJoinBytes = (kMaxGrid * 17 + 2 * kRows + kMaxGrid) * 4;
+  static_assert(kJoinBytes <= kRedBytes, "a join's statistics fit");
   static constexpr uint32_t kStatOff = kRedOff + kRedBytes;  // per warp and row
   static constexpr uint32_t kStatBytes = kWarps * kRows * 8;
   static constexpr uint32_t kBarOff = kStatOff + kStatBytes;
-  // full[stage], empty[stage]
-  static constexpr uint32_t kMiscOff = kBarOff + 2 * kStages * 8;
+  // full[stage], empty[stage], the copies of a join
+  static constexpr uint32_t kMiscOff = kBarOff + (2 * kStages + 1) * 8;
   static constexpr uint32_t kSmemBytes = kMiscOff + sizeof(PlanSmem) + 16;
   static_assert(kSmemBytes + 1024 <= 228 * 1024, "above the SM's shared memory");
-  static constexpr int kSlotFloats = kRows * (D + 2);  // a partial: O, m, l
+  static constexpr int kSlotFloats = kRows * (D + 2);  // the largest partial
 };
 
 // Barrier of the consumer warps. A warp whose wait ran out goes on through
@@ -91,92 +93,104 @@ __device__ __forceinline__ void store_result(const PagedArgs &a, const Row &w,
     a.lse[row] = l == 0.f ? -INFINITY : 0.69314718055994531f * (m + log2f(l));
 }
 
-// Joins the partials of a split item (by the CTA that finished last): the
-// CTAs' maxima and sums become weights in shared memory first, then every
-// thread adds up one row's four dims over every n-th CTA, so that all loads
-// of a step are under way together.
+// Partials of a split item lie one after the other, in the order of its
+// CTAs, from twice the first one's index on: n parts take n records, and the
+// next split item begins 2 (n - 1) further. A record: O of the item's rows,
+// then their maxima and sums, each padded to 16 bytes.
+__host__ __device__ __forceinline__ int record_floats(int d, int n_rows) {
+  return n_rows * d + 2 * ((n_rows + 3) & ~3);
+}
+
+// Joins the partials of a split item (by the CTA that finished last): weights
+// from the CTAs' maxima and sums, then every thread adds up one row's four
+// dims over every n-th CTA. Where the ring is free (the CTA's last part), one
+// bulk copy brings the records there (74 records of 7 rows x 64: 6.5 us by
+// ordinary loads, of which an SM has too few under way).
 template <int D>
 __device__ __forceinline__ void join(const PagedArgs &a, const Division &d,
                                      const Part &it, int n_rows, float *red,
-                                     int dtype) {
+                                     uint8_t *ring, uint64_t *bar, int dtype) {
   using C = Cfg<D>;
   const int tid = threadIdx.x;  // 256 consumers
   const int c0 = d.owner(it.at), n = d.owner(it.at + it.cost - 1) - c0 + 1;
-  // red: weight [CTA][row], sum and maximum per row, the CTAs' slots (-1:
-  // none of the item); later the sums of the thread groups
+  const int rec = record_floats(D, n_rows), pad = (n_rows + 3) & ~3;
+  const float *from = a.partials + 2 * static_cast<size_t>(c0) * C::kSlotFloats;
+  const bool copied = ring != nullptr && n * rec * 4 <= static_cast<int>(C::kRedOff);
+  if (copied && tid == 0) {
+    // the records were written by other SMs' ordinary stores
+    asm volatile("fence.proxy.async;" ::: "memory");
+    mbar_arrive_expect_tx(bar, n * rec * 4);
+    bulk_load(ring, from, n * rec * 4, bar, l2_policy_evict_first());
+  }
+  // red: the weight [CTA][row], maximum and sum per row, which CTAs have a
+  // part; later the sums of the thread groups
+  constexpr int kPitch = 17;
   float *weight = red;
-  float2 *total = reinterpret_cast<float2 *>(red + kMaxGrid * kRows);
-  int *slots = reinterpret_cast<int *>(total + kRows);
-  static_assert((kMaxGrid * kRows + 2 * kRows + kMaxGrid) * 4 <= C::kRedBytes,
-                "the join's statistics fit");
-  const int units = n_rows * (D / 4);
-  const int groups = max(1, 32 * kWarps / units);
+  float2 *total = reinterpret_cast<float2 *>(weight + kMaxGrid * kPitch);
+  int *has = reinterpret_cast<int *>(total + kRows);
   if (tid < n) {
     int t0, t1;
     tiles_of_cta(a, d, it, c0 + tid, t0, t1);
-    slots[tid] = t0 < t1 ? 2 * (c0 + tid) + slot_of(t0) : -1;
+    has[tid] = t0 < t1;
   }
   meet();
+  if (copied) {
+    // (a wait that runs out leaves its error and a wrong row)
+    mbar_wait(bar, 0);
+    from = reinterpret_cast<const float *>(ring);
+  }
   {
-    // sixteen threads a row
-    constexpr int kMost = (kMaxGrid + 15) / 16;
-    const int row = tid >> 4;
-    float m[kMost], l[kMost];
+    // sixteen threads a row; a part whose sum is zero saw nothing
+    const int r = tid >> 4;
+    const bool on = r < n_rows;
     float M = kNegBig, L = 0.f;
-#pragma unroll
-    for (int i = 0; i < kMost; ++i) {
-      const int c = (tid & 15) + 16 * i;
-      const int slot = c < n && row < n_rows ? slots[c] : -1;
-      const float *p = a.partials + slot * C::kSlotFloats + kRows * D + row;
-      m[i] = slot >= 0 ? __ldcg(p) : kNegBig;
-      l[i] = slot >= 0 ? __ldcg(p + kRows) : 0.f;
+#pragma unroll 4
+    for (int c = tid & 15; c < n; c += 16) {
+      const float *p = from + c * rec + n_rows * D + r;
+      if (on && has[c] && p[pad] != 0.f) M = fmaxf(M, p[0]);
     }
 #pragma unroll
-    for (int i = 0; i < kMost; ++i) {
-      if (l[i] == 0.f) m[i] = kNegBig;  // saw nothing
-      M = fmaxf(M, m[i]);
+    for (int k = 1; k < 16; k <<= 1)
+      M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+#pragma unroll 4
+    for (int c = tid & 15; c < n; c += 16) {
+      const float *p = from + c * rec + n_rows * D + r;
+      float w = 0.f;
+      if (on && has[c] && p[pad] != 0.f) {
+        w = fast_exp2(p[0] - M);
+        L = fmaf(p[pad], w, L);
+      }
+      weight[c * kPitch + r] = w;
     }
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1)
-      M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-#pragma unroll
-    for (int i = 0; i < kMost; ++i) {
-      const int c = (tid & 15) + 16 * i;
-      const float w = l[i] == 0.f ? 0.f : fast_exp2(m[i] - M);
-      if (c < n) weight[c * kRows + row] = w;
-      L = fmaf(l[i], w, L);
-    }
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    if ((tid & 15) == 0) total[row] = make_float2(M, L);
+    for (int k = 1; k < 16; k <<= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
+    if ((tid & 15) == 0) total[r] = make_float2(M, L);
   }
   meet();
+  const int units = n_rows * (D / 4);
+  const int groups = max(1, 32 * kWarps / units);
   for (int u0 = 0; u0 < units; u0 += 32 * kWarps) {
     const int g = groups > 1 ? tid / units : 0;
     const int u = groups > 1 ? tid % units : u0 + tid;
     const bool on = g < groups && u < units;
     const int row = on ? u / (D / 4) : 0, d4 = u % (D / 4);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kBatch = 16;  // loads under way
-    for (int c1 = on ? g : n; c1 < n; c1 += kBatch * groups) {
-      float4 o[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int c = c1 + i * groups;
-        const int slot = c < n ? slots[c] : -1;
-        o[i] = slot >= 0 ? __ldcg(reinterpret_cast<const float4 *>(
-                               a.partials + slot * C::kSlotFloats + row * D) + d4)
-                         : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int c = c1 + i * groups;
-        const float w = c < n ? weight[c * kRows + row] : 0.f;
-        acc.x = fmaf(o[i].x, w, acc.x);
-        acc.y = fmaf(o[i].y, w, acc.y);
-        acc.z = fmaf(o[i].z, w, acc.z);
-        acc.w = fmaf(o[i].w, w, acc.w);
-      }
+    const float4 *src = reinterpret_cast<const float4 *>(from + row * D) + d4;
+    auto add = [&](float4 o, float w) {
+      // weight zero: nothing is there, and what memory holds may be NaN
+      acc.x = w != 0.f ? fmaf(o.x, w, acc.x) : acc.x;
+      acc.y = w != 0.f ? fmaf(o.y, w, acc.y) : acc.y;
+      acc.z = w != 0.f ? fmaf(o.z, w, acc.z) : acc.z;
+      acc.w = w != 0.f ? fmaf(o.w, w, acc.w) : acc.w;
+    };
+    if (copied) {
+#pragma unroll 8
+      for (int c = on ? g : n; c < n; c += groups)
+        add(src[c * (rec / 4)], weight[c * kPitch + row]);
+    } else {
+#pragma unroll 8
+      for (int c = on ? g : n; c < n; c += groups)
+        add(__ldcg(src + c * (rec / 4)), weight[c * kPitch + row]);
     }
     const float2 ml = total[row];
     if (groups > 1) {
@@ -185,8 +199,8 @@ __device__ __forceinline__ void join(const PagedArgs &a, const Division &d,
       sums[tid] = acc;
       meet();
       if (on && g == 0) {
-        for (int o = 1; o < groups; ++o) {
-          const float4 v = sums[tid + o * units];
+        for (int k = 1; k < groups; ++k) {
+          const float4 v = sums[tid + k * units];
           acc.x += v.x;
           acc.y += v.y;
           acc.z += v.z;
@@ -204,7 +218,7 @@ __device__ __forceinline__ void join(const PagedArgs &a, const Division &d,
 
 template <int D, typename Dt>
 __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
-                        uint8_t *smem, uint64_t *full, uint64_t *empty) {
+                        uint8_t *smem, uint64_t *full, uint64_t *empty, uint64_t *copies) {
   using C = Cfg<D>;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -346,9 +360,13 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
     }
     const int group = a.H / a.H_kv;
     const int n_rows = min(a.item_tokens, it.seq.n - it.token) * group;
-    float *slot = a.partials + (2 * static_cast<size_t>(blockIdx.x) +
-                                slot_of(it.t0)) * C::kSlotFloats;
     const bool whole = it.whole();
+    float *slot = nullptr;
+    if (!whole) {
+      const int c0 = d.owner(it.at);
+      slot = a.partials + 2 * static_cast<size_t>(c0) * C::kSlotFloats +
+             static_cast<int>(blockIdx.x - c0) * record_floats(D, n_rows);
+    }
     // as many dims at a time as fit for this many rows: a power of two, 32
     // at 16 rows, all of them up to 4 rows of 128 or 8 of 64
     const int chunk = min(D, 32 << (n_rows <= 4 ? 2 : n_rows <= 8 ? 1 : 0));
@@ -386,8 +404,8 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
         } else {
           *reinterpret_cast<float2 *>(slot + r * D + dim) = sum;
           if (dim == 0) {
-            slot[kRows * D + r] = M;
-            slot[kRows * D + kRows + r] = L;
+            slot[n_rows * D + r] = M;
+            slot[n_rows * D + ((n_rows + 3) & ~3) + r] = L;
           }
         }
       }
@@ -406,7 +424,11 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
       }
       meet();
       if (threadIdx.x == 0) FA_TRACE_CTA(5);
-      if (*last) join<D>(a, d, it, n_rows, red, Dt::kDtype);
+      if (*last) {
+        // no part follows: every tile has been used
+        uint8_t *ring = walk.at >= walk.u1 ? smem : nullptr;
+        join<D>(a, d, it, n_rows, red, ring, copies, Dt::kDtype);
+      }
       if (threadIdx.x == 0) FA_TRACE_CTA(6);
       meet();
     }
@@ -423,6 +445,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   const int lane = threadIdx.x & 31;
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::kBarOff);
   uint64_t *empty = full + C::kStages;
+  uint64_t *copies = empty + C::kStages;
   PlanSmem *ps = reinterpret_cast<PlanSmem *>(smem + C::kMiscOff);
   if (threadIdx.x == 0) FA_TRACE_CTA(0);
 #ifdef FA_TRACE
@@ -440,6 +463,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         mbar_init(&full[s], C::kProducers);
         mbar_init(&empty[s], kWarps);
       }
+      mbar_init(copies, 1);
       fence_barrier_init();
       prefetch_tensormap(&tm_k);
       prefetch_tensormap(&tm_v);
@@ -449,7 +473,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   if (threadIdx.x == 0) FA_TRACE_CTA(1);
 
   if (warp < kWarps) {
-    consume<D, Dt>(a, d, walk, smem, full, empty);
+    consume<D, Dt>(a, d, walk, smem, full, empty, copies);
     return;
   }
   // ---- producers: lane j loads box j of the tile
