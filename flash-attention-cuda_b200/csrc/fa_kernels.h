@@ -141,7 +141,11 @@ struct RopeArgs {
   int64_t position_stride;
   const double *freqs;
   float amplitude, sign;
-  int tokens_per_block, rows_per_block;  // set by the launch
+  // set by the launch: how a warp's lanes lie on units and rows, the chunks
+  // that a token's rows (q's, from k_before on k's, from v_before on v's) are
+  // cut into, and from a warp's token to its next
+  int unit_lanes, row_lanes, rows_per_chunk, chunks, k_before, v_before;
+  int token_step;
   // append
   const int32_t *starts;
   const int32_t *seq_lens;
@@ -152,7 +156,7 @@ struct RopeArgs {
 };
 // vector: every row is 16-byte aligned and rotates in whole 16-byte units.
 cudaError_t launch_rope_kernel(const RopeArgs &a, bool interleaved,
-                               bool append, bool vector, int dtype,
+                               bool append, bool vector, int dtype, int sms,
                                cudaStream_t stream);
 
 // ---- attention over a paged cache (paged_attend_sm100.cu) -------------------

@@ -112,7 +112,8 @@ int fa_rope(const void *q, const int64_t q_strides[3], void *q_out,
       (reinterpret_cast<uintptr_t>(k) & 1u) ||
       (reinterpret_cast<uintptr_t>(k_out) & 1u))
     return FA_EALIGN;
-  rc = ensure_device(nullptr);
+  int dev = 0;
+  rc = ensure_device(&dev);
   if (rc != FA_OK) return rc;
 
   RopeArgs a{};
@@ -154,6 +155,7 @@ int fa_rope(const void *q, const int64_t q_strides[3], void *q_out,
                       (!k || (aligned16(k) && aligned16(k_out) &&
                               strides_vector(k_strides, k_sizes, 3)));
   return launch_rope_kernel(a, interleaved, false, vector, dtype,
+                            g_devices[dev].sms,
                             static_cast<cudaStream_t>(stream)) == cudaSuccess
              ? FA_OK
              : FA_ECUDA;
@@ -186,7 +188,8 @@ int fa_append_paged(const void *q, const int64_t q_strides[2], void *q_out,
       (reinterpret_cast<uintptr_t>(k_new) & 1u) ||
       (reinterpret_cast<uintptr_t>(v_new) & 1u))
     return FA_EALIGN;
-  rc = ensure_device(nullptr);
+  int dev = 0;
+  rc = ensure_device(&dev);
   if (rc != FA_OK) return rc;
 
   const fa_paged_cache &c = *cache;
@@ -240,6 +243,7 @@ int fa_append_paged(const void *q, const int64_t q_strides[2], void *q_out,
                       (!q || (aligned16(q) && aligned16(q_out) &&
                               strides_vector(q_strides, q_sizes, 2)));
   return launch_rope_kernel(a, interleaved, true, vector, dtype,
+                            g_devices[dev].sms,
                             static_cast<cudaStream_t>(stream)) == cudaSuccess
              ? FA_OK
              : FA_ECUDA;

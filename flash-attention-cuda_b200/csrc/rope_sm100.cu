@@ -8,9 +8,13 @@
 // the product alone would be 0.004 rad off at position 100000).
 //
 // Bound: HBM for long inputs (each element is read and written once), launch
-// latency for a generation step. A block takes a few tokens, forms their
-// cosines and sines once in shared memory (every head of a token shares
-// them) and streams the heads' rows through 16-byte accesses.
+// latency for a generation step. A warp takes tokens, and of each some or all
+// rows (heads of q, k and v). A lane keeps to one unit of the rows, 16 bytes
+// (twice, in each half, where pairs are half a head apart), so its cosines and
+// sines stay in registers for all of a token's rows. A token's
+// first loads are issued before anything else; behind them the warp finds the
+// token's cache row and forms the cosines and sines, a pair or two a lane,
+// handed round through shared memory without a block-wide barrier.
 
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -24,19 +28,10 @@
 namespace fa {
 namespace rope {
 
-constexpr int kThreads = 256;
-constexpr int kMaxTokens = 4;    // tokens of a block
-constexpr int kMaxPairs = 512;   // rotary_dim / 2 at head_dim 1024
+constexpr int kWarps = 4;       // of a block
+constexpr int kMaxPairs = 512;  // rotary_dim / 2 at head_dim 1024
 
-struct Smem {
-  float2 turn[kMaxTokens * kMaxPairs];  // (cos, sin) * amplitude
-  double position[kMaxTokens];
-  long long k_at[kMaxTokens];  // element offset of the cache row, -1: none
-  long long v_at[kMaxTokens];
-  int in_step[kMaxTokens];  // the token belongs to a sequence
-};
-
-// V consecutive 16-bit elements (16 bytes, or one).
+// V consecutive 16-bit elements.
 template <int V>
 struct Pack;
 template <>
@@ -51,10 +46,10 @@ struct Pack<1> {
 template <typename Dt, int V>
 __device__ __forceinline__ void to_float(const typename Pack<V>::T &x,
                                          float (&f)[V]) {
-  if constexpr (V == 8) {
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  if constexpr (V > 1) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&x);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < V / 2; ++i) {
       const float2 p = Dt::unpack2(w[i]);
       f[2 * i] = p.x;
       f[2 * i + 1] = p.y;
@@ -74,215 +69,260 @@ __device__ __forceinline__ typename Pack<V>::T from_float(const float (&f)[V]) {
   }
 }
 
-// One unit of a row: V elements of each half of the rotated part, V
-// neighbouring elements of it (at least one pair) with kInterleaved, or V
-// copied elements after it.
-template <typename Dt, int V, bool kInterleaved>
-__device__ __forceinline__ void move_unit(const __half *src, __half *dst,
-                                          int u, int rot, const float2 *turn) {
-  using T = typename Pack<V>::T;
-  constexpr int kPairStep = kInterleaved ? (V == 1 ? 2 : V) : V;
-  const int n_pair_units = kInterleaved ? rot / kPairStep : rot / (2 * V);
-  if (u >= n_pair_units) {
-    const int e = rot + (u - n_pair_units) * V;
-    *reinterpret_cast<T *>(dst + e) = *reinterpret_cast<const T *>(src + e);
-    return;
+// Units of a row: V elements of each half of the rotated part, or with
+// kInterleaved V neighbours of it (at least one pair), or V elements after
+// it. Where a unit's two loads are (the second -1 if it has one).
+struct Unit {
+  int first, second;
+  int pair;  // its first pair, -1: copied
+};
+template <int V, bool kInterleaved>
+struct Layout {
+  static constexpr int kWide = kInterleaved && V == 1 ? 2 : V;  // elements
+  __host__ __device__ static int pair_units(int rot) {
+    return kInterleaved ? rot / kWide : rot / (2 * V);
   }
-  const int e = u * kPairStep;
-  if constexpr (kInterleaved && V == 1) {
-    float a[1], b[1];
-    to_float<Dt, 1>(src[e], a);
-    to_float<Dt, 1>(src[e + 1], b);
-    const float2 t = turn[u];
-    const float y0[1] = {a[0] * t.x - b[0] * t.y};
-    const float y1[1] = {b[0] * t.x + a[0] * t.y};
-    dst[e] = from_float<Dt, 1>(y0);
-    dst[e + 1] = from_float<Dt, 1>(y1);
-  } else if constexpr (kInterleaved) {
-    float f[V], y[V];
-    to_float<Dt, V>(*reinterpret_cast<const T *>(src + e), f);
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      const float2 t = turn[e / 2 + i];
-      y[2 * i] = f[2 * i] * t.x - f[2 * i + 1] * t.y;
-      y[2 * i + 1] = f[2 * i + 1] * t.x + f[2 * i] * t.y;
-    }
-    *reinterpret_cast<T *>(dst + e) = from_float<Dt, V>(y);
-  } else {
-    const int half = rot / 2;
-    float a[V], b[V], y0[V], y1[V];
-    to_float<Dt, V>(*reinterpret_cast<const T *>(src + e), a);
-    to_float<Dt, V>(*reinterpret_cast<const T *>(src + half + e), b);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float2 t = turn[e + i];
-      y0[i] = a[i] * t.x - b[i] * t.y;
-      y1[i] = b[i] * t.x + a[i] * t.y;
-    }
-    *reinterpret_cast<T *>(dst + e) = from_float<Dt, V>(y0);
-    *reinterpret_cast<T *>(dst + half + e) = from_float<Dt, V>(y1);
+  __host__ __device__ static int units(int d, int rot) {
+    return pair_units(rot) + (d - rot) / V;
   }
-}
+  __device__ static Unit unit(int u, int rot) {
+    const int n = pair_units(rot);
+    if (u >= n) return {rot + (u - n) * V, -1, -1};
+    if (!kInterleaved) return {u * V, rot / 2 + u * V, u * V};
+    return {u * kWide, kWide > V ? u * kWide + 1 : -1, u * kWide / 2};
+  }
+};
 
-// Where token t of a step is: its row in its sequence's cache (and through
-// the page table, the element offsets of that row). Called by a whole warp.
-__device__ __forceinline__ void place_token(const RopeArgs &a, int t, int slot,
-                                            Smem &s) {
+// Where token t of a step is: its row's position, and the element offsets of
+// that row in the pools (-1: it is not stored). False: it is no sequence's.
+// Called by a whole warp.
+__device__ __forceinline__ bool place_token(const RopeArgs &a, int t,
+                                            double &position, long long &k_at,
+                                            long long &v_at) {
   const int lane = threadIdx.x & 31;
-  // the sequences that end at or before t come before t's own
-  int seq = 0;
-  for (int b = lane; b < a.batch; b += 32) seq += a.starts[b + 1] <= t;
-  seq = __reduce_add_sync(0xffffffffu, seq);
-  if (lane != 0) return;
-  s.k_at[slot] = s.v_at[slot] = -1;
-  s.in_step[slot] = seq < a.batch;
-  s.position[slot] = 0.;
-  if (seq >= a.batch) return;
+  // the sequences that end at or before t come before its own: counted in
+  // steps first, then one by one in the step that is left
+  const int step = (a.batch + 31) >> 5;
+  const int at = (lane + 1) * step;
+  int seq = step * __popc(__ballot_sync(0xffffffffu, at <= a.batch && a.starts[at] <= t));
+  const int end = min(seq + step, a.batch);
+  int more = 0;
+  for (int b = seq + lane; step > 1 && b < end; b += 32) more += a.starts[b + 1] <= t;
+  seq += __reduce_add_sync(0xffffffffu, more);
+  position = 0.;
+  k_at = v_at = -1;
+  if (seq >= a.batch) return false;
   const long long row =
       static_cast<long long>(a.seq_lens[seq]) - a.starts[seq + 1] + t;
-  s.position[slot] = a.positions ? static_cast<double>(a.positions[t])
-                                 : static_cast<double>(row);
+  position = a.positions ? static_cast<double>(a.positions[t])
+                         : static_cast<double>(row);
   if (row < 0 || row >= static_cast<long long>(a.table_width) * a.page_rows)
-    return;
-  const int page = a.page_table[seq * a.table_stride + row / a.page_rows];
+    return true;
+  const uint32_t index = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.page_rows);
+  const int page = a.page_table[seq * a.table_stride + index];
   if (page < 0 || page >= a.num_pages) {
-    record_error(FA_ERR_PAGE);
-    return;
+    if (lane == 0) record_error(FA_ERR_PAGE);
+    return true;
   }
-  const long long r = row % a.page_rows;
-  s.k_at[slot] = page * a.kp_sp + r * a.kp_sr;
-  s.v_at[slot] = page * a.vp_sp + r * a.vp_sr;
+  const long long r = row - static_cast<long long>(index) * a.page_rows;
+  k_at = page * a.kp_sp + r * a.kp_sr;
+  v_at = page * a.vp_sp + r * a.vp_sr;
+  return true;
 }
 
-// Block (x, y): tokens [x * tokens_per_block, ...), rows (heads of q, then k,
-// then v) [y * rows_per_block, ...).
-template <typename Dt, int V, bool kInterleaved, bool kAppend>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const RopeArgs a) {
-  __shared__ Smem s;
-  const int t0 = static_cast<int>(blockIdx.x) * a.tokens_per_block;
-  const int n_tok = min(a.tokens_per_block, a.tokens - t0);
-  const int pairs = a.rot / 2;
-  if (kAppend) {
-    for (int i = threadIdx.x >> 5; i < n_tok; i += kThreads / 32)
-      place_token(a, t0 + i, i, s);
-    __syncthreads();
-  }
-  for (int i = threadIdx.x; i < n_tok * pairs; i += kThreads) {
-    const int tok = i / pairs;
-    double p;
-    if (kAppend) {
-      p = s.position[tok];
-    } else {
-      const int t = t0 + tok;
-      p = a.positions[(t / a.N) * a.position_stride + t % a.N];
-    }
-    double turns = p * a.freqs[i - tok * pairs] * 0.15915494309189533577;
-    turns -= rint(turns);
-    float sn, cs;
-    sincospif(static_cast<float>(2. * turns), &sn, &cs);
-    s.turn[i] = make_float2(cs * a.amplitude, sn * a.amplitude * a.sign);
-  }
-  __syncthreads();
+constexpr double kTurnsPerRadian = 0.15915494309189533577;
 
-  const int pair_units = kInterleaved ? a.rot / (V == 1 ? 2 : V) : a.rot / (2 * V);
-  const int units = pair_units + (a.D - a.rot) / V;
-  const int all_rows = a.H + a.H_kv + (kAppend ? a.H_kv : 0);
-  const int row0 = static_cast<int>(blockIdx.y) * a.rows_per_block;
-  const int n_rows = min(a.rows_per_block, all_rows - row0);
-  for (int i = threadIdx.x; i < n_tok * n_rows * units; i += kThreads) {
-    const int u = i % units;
-    const int rest = i / units;
-    const int tok = rest / n_rows;
-    const int row = row0 + rest - tok * n_rows;
-    const int t = t0 + tok;
+// (cos, sin) of a fraction of a turn. The fast sine and cosine are good to
+// 2^-21 in this range, far below a 16-bit result's rounding.
+__device__ __forceinline__ float2 turn_of(const RopeArgs &a, float fraction) {
+  float sn, cs;
+  __sincosf(fraction * 6.2831853071795865f, &sn, &cs);
+  return make_float2(cs * a.amplitude, sn * a.amplitude * a.sign);
+}
+
+// Rows of a lane under way, 64 bytes either way.
+template <bool kInterleaved>
+__host__ __device__ constexpr int batch_rows() {
+  return kInterleaved ? 4 : 2;
+}
+
+// Warp w of the grid: chunk w % chunks of the rows (heads of q, then k, then
+// v) of tokens w / chunks, w / chunks + token_step, ...
+template <typename Dt, int V, bool kInterleaved, bool kAppend>
+__global__ void __launch_bounds__(32 * kWarps) rope_kernel(const RopeArgs a) {
+  constexpr int kBatch = batch_rows<kInterleaved>();
+  using L = Layout<V, kInterleaved>;
+  using T = typename Pack<V>::T;
+  __shared__ float2 turns_of[kWarps][kMaxPairs];  // (cos, sin) * amplitude
+  float2 *turns = turns_of[threadIdx.x >> 5];
+  const int lane = threadIdx.x & 31;
+  const uint32_t w = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int first_token = static_cast<int>(w / static_cast<uint32_t>(a.chunks));
+  const int chunk = static_cast<int>(w) - first_token * a.chunks;
+  // lanes: units along a row (or 32 of them at a time), then rows
+  const int units = L::units(a.D, a.rot);
+  const int row_lane = lane / a.unit_lanes;
+  const int ux = lane - row_lane * a.unit_lanes;
+  // the chunk's rows of q, k and v, as [begin, end) of each
+  const int all0 = chunk * a.rows_per_chunk;
+  const int all1 = all0 + a.rows_per_chunk;
+  constexpr int kSections = kAppend ? 3 : 2;
+  for (int t = first_token; t < a.tokens; t += a.token_step) {
     const int b = kAppend ? 0 : t / a.N;
     const int n = kAppend ? t : t - b * a.N;
-    if (kAppend && !s.in_step[tok]) continue;
-    const __half *src;
-    __half *dst;
-    if (row < a.H) {
-      src = a.q + b * a.q_sb + row * a.q_sh + n * a.q_sn;
-      dst = a.q_out + b * a.qo_sb + row * a.qo_sh + n * a.qo_sn;
-    } else if (row < a.H + a.H_kv) {
-      const int h = row - a.H;
-      src = a.k + b * a.k_sb + h * a.k_sh + n * a.k_sn;
-      if (kAppend) {
-        if (s.k_at[tok] < 0) continue;
-        dst = a.k_out + s.k_at[tok] + h * a.kp_sh;
-      } else {
-        dst = a.k_out + b * a.ko_sb + h * a.ko_sh + n * a.ko_sn;
+    double position = 0.;
+    long long k_at = 0, v_at = 0;
+    bool ready = false, skip = false;
+#pragma unroll 1
+    for (int sec = 0; sec < kSections; ++sec) {
+      const int before = sec == 0 ? 0 : sec == 1 ? a.k_before : a.v_before;
+      const int row1 = row_lane < a.row_lanes
+                           ? min(all1 - before, sec == 0 ? a.H : a.H_kv)
+                           : 0;
+      const int begin = max(all0 - before, 0);
+      if (begin >= min(all1 - before, sec == 0 ? a.H : a.H_kv)) continue;
+      const int row0 = begin + row_lane;
+      const __half *src = sec == 0   ? a.q + b * a.q_sb + n * a.q_sn
+                          : sec == 1 ? a.k + b * a.k_sb + n * a.k_sn
+                                     : a.v + n * a.v_sn;
+      int64_t sh = sec == 0 ? a.q_sh : sec == 1 ? a.k_sh : a.v_sh;
+      src += row0 * sh;
+      sh *= a.row_lanes;
+      T x[kBatch], y[kBatch];
+      auto load = [&](const Unit &unit, const __half *from, int r) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          if (r + i * a.row_lanes >= row1) continue;
+          x[i] = *reinterpret_cast<const T *>(from + unit.first);
+          if (unit.second >= 0) y[i] = *reinterpret_cast<const T *>(from + unit.second);
+          from += sh;
+        }
+      };
+      if (ux < units) load(L::unit(ux, a.rot), src, row0);
+
+      if (!ready) {
+        ready = true;
+        if (kAppend)
+          skip = !place_token(a, t, position, k_at, v_at);
+        else
+          position = a.positions[b * a.position_stride + n];
+        __syncwarp();  // the last token's cosines and sines have been read
+        for (int i = lane; i < a.rot / 2; i += 32) {
+          const double turns_all = position * a.freqs[i] * kTurnsPerRadian;
+          turns[i] = turn_of(a, static_cast<float>(turns_all - rint(turns_all)));
+        }
+        __syncwarp();
       }
-    } else {
-      const int h = row - a.H - a.H_kv;
-      if (s.v_at[tok] < 0) continue;
-      src = a.v + h * a.v_sh + n * a.v_sn;
-      dst = a.v_out + s.v_at[tok] + h * a.vp_sh;
-    }
-    if (kAppend && row >= a.H + a.H_kv) {
-      // V rows are copied: the same units, unrotated
-      using T = typename Pack<V>::T;
-      if constexpr (kInterleaved && V == 1) {
-        if (u < pair_units) {
-          dst[2 * u] = src[2 * u];
-          dst[2 * u + 1] = src[2 * u + 1];
-          continue;
+      if (skip || (kAppend && sec > 0 && k_at < 0)) break;
+
+      __half *dst = sec == 0 ? a.q_out + b * a.qo_sb + n * a.qo_sn
+                    : kAppend ? (sec == 1 ? a.k_out + k_at : a.v_out + v_at)
+                              : a.k_out + b * a.ko_sb + n * a.ko_sn;
+      int64_t dh = sec == 0 ? a.qo_sh : !kAppend ? a.ko_sh : sec == 1 ? a.kp_sh : a.vp_sh;
+      dst += row0 * dh;
+      dh *= a.row_lanes;
+      for (int u = ux; u < units; u += a.unit_lanes) {
+        const Unit unit = L::unit(u, a.rot);
+        const bool turned = unit.pair >= 0 && sec < 2;
+        // the unit's pairs
+        constexpr int kPairs = kInterleaved && V > 1 ? V / 2 : V;
+        float2 turn[kPairs];
+        if (turned) {
+#pragma unroll
+          for (int e = 0; e < kPairs; ++e) turn[e] = turns[unit.pair + e];
+        }
+        const __half *from = src;
+        __half *to = dst;
+        for (int r = row0; r < row1; r += kBatch * a.row_lanes) {
+          if (u != ux || r != row0) load(unit, from, r);
+          from += kBatch * sh;
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            if (r + i * a.row_lanes >= row1) continue;
+            if (turned) {
+              float f[V], g[V], p[V], o[V];
+              to_float<Dt, V>(x[i], f);
+              if constexpr (kInterleaved && V > 1) {
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) {
+                  p[2 * e] = f[2 * e] * turn[e].x - f[2 * e + 1] * turn[e].y;
+                  p[2 * e + 1] = f[2 * e + 1] * turn[e].x + f[2 * e] * turn[e].y;
+                }
+              } else {
+                to_float<Dt, V>(y[i], g);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                  p[e] = f[e] * turn[e].x - g[e] * turn[e].y;
+                  o[e] = g[e] * turn[e].x + f[e] * turn[e].y;
+                }
+                y[i] = from_float<Dt, V>(o);
+              }
+              x[i] = from_float<Dt, V>(p);
+            }
+            *reinterpret_cast<T *>(to + unit.first) = x[i];
+            if (unit.second >= 0) *reinterpret_cast<T *>(to + unit.second) = y[i];
+            to += dh;
+          }
         }
       }
-      const int e = kInterleaved || u < pair_units
-                        ? u * V
-                        : a.rot + (u - pair_units) * V;
-      if constexpr (kInterleaved && V == 1) {
-        dst[a.rot + u - pair_units] = src[a.rot + u - pair_units];
-      } else {
-        *reinterpret_cast<T *>(dst + e) = *reinterpret_cast<const T *>(src + e);
-        if (!kInterleaved && u < pair_units)
-          *reinterpret_cast<T *>(dst + a.rot / 2 + e) =
-              *reinterpret_cast<const T *>(src + a.rot / 2 + e);
-      }
-      continue;
     }
-    move_unit<Dt, V, kInterleaved>(src, dst, u, a.rot,
-                                   s.turn + tok * pairs);
   }
 }
 
 template <typename Dt, int V, bool kInterleaved, bool kAppend>
-cudaError_t launch(const RopeArgs &args, cudaStream_t stream) {
+cudaError_t launch(const RopeArgs &args, int sms, cudaStream_t stream) {
   RopeArgs a = args;
-  const int rows = a.H + a.H_kv + (kAppend ? a.H_kv : 0);
-  a.tokens_per_block = a.tokens > 4 * 148 ? kMaxTokens : 1;
-  a.rows_per_block = rows;
-  const int units = a.D / V;
-  if (a.tokens_per_block == 1) {
-    a.rows_per_block = kThreads / units > 0 ? kThreads / units : 1;
-    if (a.rows_per_block > rows) a.rows_per_block = rows;
+  const int rows = a.H + a.H_kv * (kAppend ? 2 : 1);
+  const int units = Layout<V, kInterleaved>::units(a.D, a.rot);
+  a.unit_lanes = units < 32 ? units : 32;
+  a.row_lanes = 32 / a.unit_lanes;
+  // While there are fewer tokens than warps wanted (64 an SM), a token's rows
+  // go to several, each with rows of one tensor, down to one row a lane; from
+  // more tokens than that on, a warp takes several tokens.
+  long long want = 64ll * sms;
+  const int most = a.H > a.H_kv ? a.H : a.H_kv;
+  const int steps = (most + a.row_lanes - 1) / a.row_lanes;
+  long long cuts = (want + a.tokens - 1) / a.tokens;
+  a.rows_per_chunk = rows;
+  a.k_before = a.H;
+  a.v_before = a.H + a.H_kv;
+  if (cuts > 1) {
+    if (cuts > steps) cuts = steps;
+    const int r = static_cast<int>((steps + cuts - 1) / cuts) * a.row_lanes;
+    a.rows_per_chunk = r;
+    a.k_before = (a.H + r - 1) / r * r;
+    a.v_before = a.k_before + (a.H_kv + r - 1) / r * r;
   }
-  const dim3 grid((a.tokens + a.tokens_per_block - 1) / a.tokens_per_block,
-                  (rows + a.rows_per_block - 1) / a.rows_per_block);
-  rope_kernel<Dt, V, kInterleaved, kAppend><<<grid, kThreads, 0, stream>>>(a);
+  const int end = (kAppend ? a.v_before : a.k_before) + a.H_kv;
+  a.chunks = (end + a.rows_per_chunk - 1) / a.rows_per_chunk;
+  want /= a.chunks;
+  a.token_step = static_cast<int>(want > a.tokens ? a.tokens : want < 1 ? 1 : want);
+  const long long warps = static_cast<long long>(a.token_step) * a.chunks;
+  const unsigned grid = static_cast<unsigned>((warps + kWarps - 1) / kWarps);
+  rope_kernel<Dt, V, kInterleaved, kAppend><<<grid, 32 * kWarps, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
-template <typename Dt, int V>
-cudaError_t pick(const RopeArgs &a, bool interleaved, bool append,
+template <typename Dt, bool kAppend>
+cudaError_t pick(const RopeArgs &a, bool interleaved, bool vector, int sms,
                  cudaStream_t stream) {
   if (interleaved)
-    return append ? launch<Dt, V, true, true>(a, stream)
-                  : launch<Dt, V, true, false>(a, stream);
-  return append ? launch<Dt, V, false, true>(a, stream)
-                : launch<Dt, V, false, false>(a, stream);
+    return vector ? launch<Dt, 8, true, kAppend>(a, sms, stream)
+                  : launch<Dt, 1, true, kAppend>(a, sms, stream);
+  return vector ? launch<Dt, 8, false, kAppend>(a, sms, stream)
+                : launch<Dt, 1, false, kAppend>(a, sms, stream);
 }
 
 }  // namespace rope
 
 cudaError_t launch_rope_kernel(const RopeArgs &a, bool interleaved,
-                               bool append, bool vector, int dtype,
+                               bool append, bool vector, int dtype, int sms,
                                cudaStream_t stream) {
   if (dtype == FA_DTYPE_BF16)
-    return vector ? rope::pick<BF16, 8>(a, interleaved, append, stream)
-                  : rope::pick<BF16, 1>(a, interleaved, append, stream);
-  return vector ? rope::pick<F16, 8>(a, interleaved, append, stream)
-                : rope::pick<F16, 1>(a, interleaved, append, stream);
+    return append ? rope::pick<BF16, true>(a, interleaved, vector, sms, stream)
+                  : rope::pick<BF16, false>(a, interleaved, vector, sms, stream);
+  return append ? rope::pick<F16, true>(a, interleaved, vector, sms, stream)
+                : rope::pick<F16, false>(a, interleaved, vector, sms, stream);
 }
 
 }  // namespace fa
