@@ -140,6 +140,15 @@ __device__ __forceinline__ float2 turn_of(const RopeArgs &a, float fraction) {
   return make_float2(cs * a.amplitude, sn * a.amplitude * a.sign);
 }
 
+// A pair turned, with the roundings spelled out: every layout and alignment of
+// the rows gives the same bits.
+__device__ __forceinline__ float turned_first(float a, float b, float2 t) {
+  return __fmaf_rn(a, t.x, -__fmul_rn(b, t.y));
+}
+__device__ __forceinline__ float turned_second(float a, float b, float2 t) {
+  return __fmaf_rn(b, t.x, __fmul_rn(a, t.y));
+}
+
 // Rows of a lane under way, 64 bytes either way.
 template <bool kInterleaved>
 __host__ __device__ constexpr int batch_rows() {
@@ -245,15 +254,15 @@ __global__ void __launch_bounds__(32 * kWarps) rope_kernel(const RopeArgs a) {
               if constexpr (kInterleaved && V > 1) {
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) {
-                  p[2 * e] = f[2 * e] * turn[e].x - f[2 * e + 1] * turn[e].y;
-                  p[2 * e + 1] = f[2 * e + 1] * turn[e].x + f[2 * e] * turn[e].y;
+                  p[2 * e] = turned_first(f[2 * e], f[2 * e + 1], turn[e]);
+                  p[2 * e + 1] = turned_second(f[2 * e], f[2 * e + 1], turn[e]);
                 }
               } else {
                 to_float<Dt, V>(y[i], g);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                  p[e] = f[e] * turn[e].x - g[e] * turn[e].y;
-                  o[e] = g[e] * turn[e].x + f[e] * turn[e].y;
+                  p[e] = turned_first(f[e], g[e], turn[e]);
+                  o[e] = turned_second(f[e], g[e], turn[e]);
                 }
                 y[i] = from_float<Dt, V>(o);
               }
