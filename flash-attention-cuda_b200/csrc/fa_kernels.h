@@ -177,7 +177,7 @@ struct PagedArgs {
   int causal;
   // set by the launch: rows of a TMA box, new tokens of an item, and the
   // division of the work (paged_sm100.cuh)
-  int box_rows, item_tokens, item_cost, min_piece, min_part;
+  int box_rows, item_tokens, item_cost, min_piece, min_part, whole_tiles;
   float *partials;
   uint32_t *counters;
 };

@@ -71,18 +71,20 @@ int attend_paged_form(const PagedArgs &a) {
 void attend_paged_plan(PagedArgs &a, int form) {
   const int group = a.H / a.H_kv;
   a.box_rows = paged::box_rows(a.page_rows);
-  a.min_part = 1;
+  a.min_part = 2;
   if (form == kPagedFew) {
     a.item_tokens = paged::few::kRows / group;
     a.item_cost = 384;
-    a.min_piece = 640;
+    a.min_piece = 400;
+    a.whole_tiles = 7;
   } else {
     a.item_tokens = 2 * (paged::many::kRows / group);
-    a.item_cost = 256;
-    a.min_piece = 512;
-    a.min_part = 2;
+    a.item_cost = 384;
+    a.min_piece = 384;
+    a.whole_tiles = 1;
   }
 #ifdef FA_TUNE
+  if (getenv("FA_WHOLE")) a.whole_tiles = atoi(getenv("FA_WHOLE"));
   if (getenv("FA_PART")) a.min_part = atoi(getenv("FA_PART"));
   if (getenv("FA_COST")) a.item_cost = atoi(getenv("FA_COST"));
   if (getenv("FA_PIECE")) a.min_piece = atoi(getenv("FA_PIECE"));

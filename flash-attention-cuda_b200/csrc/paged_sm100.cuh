@@ -136,14 +136,16 @@ __host__ __device__ __forceinline__ int tiles_of(int keys) {
 }
 
 // The first tile that a position inside an item leaves to its right. Parts of
-// less than a.min_part tiles cost more than the balance they bring: such a
-// position moves to the item's start or end.
+// less than a.min_part tiles, and splits of items of up to a.whole_tiles, cost
+// more than the balance they bring: such a position moves to the nearer end of
+// the item.
 __host__ __device__ __forceinline__ int tile_at(const PagedArgs &a, int tiles,
                                                 long long x) {
   const long long k = x - a.item_cost;
   if (k <= 0) return 0;
   // k is at most an item's keys, so it fits 32 bits
   const int t = static_cast<int>((static_cast<uint32_t>(k) + kTileKeys - 1) / kTileKeys);
+  if (tiles <= a.whole_tiles) return 2 * t < tiles ? 0 : tiles;
   return t < a.min_part ? 0 : t > tiles - a.min_part ? tiles : t;
 }
 
