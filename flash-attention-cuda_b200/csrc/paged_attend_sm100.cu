@@ -83,12 +83,6 @@ void attend_paged_plan(PagedArgs &a, int form) {
     a.min_piece = 384;
     a.whole_tiles = 1;
   }
-#ifdef FA_TUNE
-  if (getenv("FA_WHOLE")) a.whole_tiles = atoi(getenv("FA_WHOLE"));
-  if (getenv("FA_PART")) a.min_part = atoi(getenv("FA_PART"));
-  if (getenv("FA_COST")) a.item_cost = atoi(getenv("FA_COST"));
-  if (getenv("FA_PIECE")) a.min_piece = atoi(getenv("FA_PIECE"));
-#endif
 }
 
 cudaError_t launch_attend_paged_kernel(const PagedArgs &a, int form,

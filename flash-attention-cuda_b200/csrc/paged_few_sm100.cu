@@ -261,7 +261,6 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
         ok = false;
         break;
       }
-      if (threadIdx.x == 0 && pos == 0) FA_TRACE_CTA(2);
       const int base = i * kTileKeys;
       // rows of this warp that the tile holds
       const int here = min(it.keys - base, kTileKeys) - key0;
@@ -349,7 +348,6 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
     }
 
     // ---- the warps' states, joined
-    if (threadIdx.x == 0) FA_TRACE_CTA(3);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
@@ -412,7 +410,6 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
       if (!whole && d0 + chunk == D) __threadfence();
       meet();
     }
-    if (threadIdx.x == 0) FA_TRACE_CTA(4);
     if (!whole) {
       // the part that completes the item's tiles joins them
       uint32_t *counter = a.counters + d.owner(it.at);
@@ -423,13 +420,11 @@ __device__ void consume(const PagedArgs &a, const Division &d, Walk &walk,
         __threadfence();
       }
       meet();
-      if (threadIdx.x == 0) FA_TRACE_CTA(5);
       if (*last) {
         // no part follows: every tile has been used
         uint8_t *ring = walk.at >= walk.u1 ? smem : nullptr;
         join<D>(a, d, it, n_rows, red, ring, copies, Dt::kDtype);
       }
-      if (threadIdx.x == 0) FA_TRACE_CTA(6);
       meet();
     }
   }
@@ -447,10 +442,6 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   uint64_t *empty = full + C::kStages;
   uint64_t *copies = empty + C::kStages;
   PlanSmem *ps = reinterpret_cast<PlanSmem *>(smem + C::kMiscOff);
-  if (threadIdx.x == 0) FA_TRACE_CTA(0);
-#ifdef FA_TRACE
-  if (threadIdx.x == 0) { uint32_t sm; asm volatile("mov.u32 %0, %%smid;" : "=r"(sm)); g_fa_trace[blockIdx.x * 8 + 7] = sm; }
-#endif
   if (smem_u32(smem) & 1023u) {
     if (threadIdx.x == 0) record_error(FA_ERR_SMEM_ALIGN);
     return;
@@ -470,7 +461,6 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     }
   });
   if (!work) return;
-  if (threadIdx.x == 0) FA_TRACE_CTA(1);
 
   if (warp < kWarps) {
     consume<D, Dt>(a, d, walk, smem, full, empty, copies);

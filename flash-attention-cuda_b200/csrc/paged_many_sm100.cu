@@ -10,7 +10,9 @@
 // the key tiles of one K/V head, each tile of keys loaded once for both:
 // S_t = Q_t K^T and O_t += P_t V_t by tcgen05, S and O in tensor memory, P
 // written over S as 16-bit values. The two tiles take turns, so the tensor
-// cores work on one while the other's softmax runs. One CTA per SM walks its
+// cores work on one while the other's softmax runs. Where an item has one tile
+// only, its key tiles alternate between the two softmax groups instead (at
+// D 64), each with its own state (S_t, O_t, m, l), joined at the end. One CTA per SM walks its
 // piece of the step (paged_sm100.cuh); nothing of it starts over between
 // items: the next item's queries and keys load while this one ends.
 //
@@ -74,13 +76,16 @@ struct Cfg {
   static constexpr int kPFull = kSFull + 2;          // + tile
   static constexpr int kODone = kPFull + 2;          // + tile
   static constexpr int kJoin = kODone + 2;           // + tile
-  static constexpr int kPartFull = kJoin + 2;        // + slot
+  static constexpr int kMix = kJoin + 2;             // tile 1's state is there
+  static constexpr int kMixed = kMix + 1;            // and has been taken
+  static constexpr int kPartFull = kMixed + 1;       // + slot
   static constexpr int kPartEmpty = kPartFull + kParts;  // + slot
   static constexpr int kDrain = kPartEmpty + kParts;
   static constexpr int kBars = kDrain + 1;
   static constexpr uint32_t kMiscOff = kBarOff + kBars * 8;
   static constexpr uint32_t kCtrlOff = kMiscOff + sizeof(PlanSmem);
-  static constexpr uint32_t kSmemBytes = kCtrlOff + 512;
+  static constexpr uint32_t kMixOff = kCtrlOff + 512;  // (m, l) per row
+  static constexpr uint32_t kSmemBytes = kMixOff + kRows * 8;
   static_assert(kSmemBytes + 1024 <= 228 * 1024, "above the SM's shared memory");
   static constexpr uint32_t kTmemO = 256;  // + D * tile
   // a partial of one tile: O as [D / 4][row] float4, then m and l per row
@@ -128,6 +133,7 @@ struct Job {
   int keys;        // rows of the sequence in the cache
   int tiles, t0, t1;  // key tiles of the item and of this part
   int end[2];      // of t0 .. t1, where each query tile's end
+  bool split;      // one query tile, whose key tiles both softmax groups share
   long long at, cost;
   __device__ bool whole() const { return t0 == 0 && t1 == tiles; }
 };
@@ -193,6 +199,9 @@ __device__ void hand_out(const PagedArgs &a, Walk &walk, uint64_t *bars, Ctrl *c
                             ? 0 : tiles_of(job_seen(a, j, last));
         j.end[t] = max(it.t0, min(it.t1, end));
       }
+      // (a ring of two stages cannot feed two groups apart: at D 128 this
+      // took 133 us where tile by tile takes 111, at 64 67 against 90)
+      j.split = C::kStages > 2 && j.n <= tile_tokens(a) && it.t1 - it.t0 >= 2;
     }
     mbar_arrive(&bars[C::kPartFull + n % kParts]);
     if (!more) return;
@@ -288,9 +297,9 @@ __device__ void issue(const PagedArgs &a, uint8_t *smem, uint64_t *bars, Ctrl *c
   const uint32_t sbase = smem_u32(smem);
   const uint64_t desc0 = sw128_desc(sbase);
   const uint64_t vdesc0 = v_desc<D>(sbase);
-  auto s_tile = [&](int t, int pos) {
+  auto s_tile = [&](int t, int pos, int q) {
     if (leader) {
-      issue_s<D, Dt>(tmem + 128 * t, desc0 + ((C::kQOff + t * C::kTile) >> 4),
+      issue_s<D, Dt>(tmem + 128 * t, desc0 + ((C::kQOff + q * C::kTile) >> 4),
                      desc0 + ((C::kRingOff + pos % C::kStages * C::kStage) >> 4));
       mma_commit(&bars[C::kSFull + t]);
     }
@@ -305,8 +314,45 @@ __device__ void issue(const PagedArgs &a, uint8_t *smem, uint64_t *bars, Ctrl *c
     if (!job || job->b < 0) break;
     const int t0 = job->t0, t1 = job->t1;
     const int end[2] = {job->end[0], job->end[1]};
+    const bool split = job->split;
     release<D>(bars, n);
     if (t0 >= t1) continue;
+    if (split) {
+      // key tile j goes to softmax group (j - t0) % 2; both read Q_0
+      ok = mbar_wait(&bars[C::kQFull + 0], q_used[0] & 1);
+      ++q_used[0];
+      for (int j = t0 - 2; ok && j < t1; ++j) {
+        const int t = (j - t0) & 1;
+        if (ctrl->abort) ok = false;
+        if (ok && j >= t0) {  // P V of tile j
+          const int slot = pos % C::kStages;
+          ok = mbar_wait(&bars[C::kPFull + t], done[t] & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+            issue_pv<D, Dt>(tmem + C::kTmemO + D * t, tmem + 128 * t,
+                            vdesc0 + ((C::kRingOff + slot * C::kStage + C::kTile) >> 4),
+                            j >= t0 + 2);
+            mma_commit(&bars[C::kODone + t]);
+            mma_commit(&bars[C::kEmpty + slot]);
+          }
+          __syncwarp();
+          ++done[t];
+          ++pos;
+        }
+        if (ok && j + 2 < t1) {  // S of tile j + 2, over P of tile j
+          const int p2 = pos + (j >= t0 ? 1 : j + 2 - t0);
+          ok = mbar_wait(&bars[C::kFull + p2 % C::kStages], (p2 / C::kStages) & 1) &&
+               (done[t] == 0 || mbar_wait(&bars[C::kODone + t], (done[t] - 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+          s_tile(t, p2, 0);
+          if (leader && j + 3 == t1) mma_commit(&bars[C::kQEmpty + 0]);
+          __syncwarp();
+        }
+      }
+      continue;
+    }
     // first S of each tile; its tensor memory was P of the last item
     for (int t = 0; ok && t < 2; ++t) {
       if (end[t] <= t0) continue;
@@ -316,7 +362,7 @@ __device__ void issue(const PagedArgs &a, uint8_t *smem, uint64_t *bars, Ctrl *c
       if (!ok) break;
       ++q_used[t];
       tc_fence_after();
-      s_tile(t, pos);
+      s_tile(t, pos, t);
       if (leader && end[t] == t0 + 1) mma_commit(&bars[C::kQEmpty + t]);
       __syncwarp();
     }
@@ -353,7 +399,7 @@ __device__ void issue(const PagedArgs &a, uint8_t *smem, uint64_t *bars, Ctrl *c
             continue;
           }
           tc_fence_after();
-          s_tile(t, p1);
+          s_tile(t, p1, t);
           if (leader && j + 2 == end[t]) mma_commit(&bars[C::kQEmpty + t]);
           __syncwarp();
         }
@@ -406,7 +452,7 @@ __device__ __forceinline__ void store_dims(__half *dst, const uint32_t (&o)[32],
 
 // One query tile's softmax and results. Returns false if a wait ran out.
 template <int D, typename Dt>
-__device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
+__device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl, float2 *mix) {
   using C = Cfg<D>;
   const int warp = threadIdx.x >> 5;
   const int t = warp >> 2;
@@ -415,11 +461,8 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
   const uint32_t tS = ctrl->tmem + lane_addr + 128 * t;
   const uint32_t tO = ctrl->tmem + lane_addr + C::kTmemO + D * t;
   const int group = a.H / a.H_kv;
-  // this row's token within the item, -1 for none (the tile's last rows where
-  // the group does not divide it)
-  const int tok = row / group < tile_tokens(a) ? t * tile_tokens(a) + row / group : -1;
-  int done = 0;  // key tiles of this query tile so far
-  uint32_t met = 0;
+  int done = 0;  // key tiles of this group so far
+  uint32_t met = 0, mixes = 0;
   // the tile's 128 threads meet (bounded, like every wait here)
   auto meet = [&]() {
     mbar_arrive(&bars[C::kJoin + t]);
@@ -431,23 +474,32 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
     const Job *job = take<D>(ctrl, bars, n);
     if (!job) return false;
     if (job->b < 0) return true;
-    const int t0 = job->t0, end = job->end[t];
+    const int t0 = job->t0;
+    const bool split = job->split;
+    if (t == 1 && !split && job->n <= tile_tokens(a)) continue;  // no row
+    // this row's token within the item, -1 for none (the tile's last rows
+    // where the group does not divide it)
+    const int first = split ? 0 : t * tile_tokens(a);
+    const int tok = row / group < tile_tokens(a) ? first + row / group : -1;
     const bool real = tok >= 0 && tok < job->n;
     const int seen = real ? job_seen(a, *job, tok) : 0;
     // a warp without a row only keeps the tile's barriers going
     const bool idle = !__any_sync(0xffffffffu, real);
     // keys that every row of the tile sees
-    const int all_see = job_seen(a, *job, t * tile_tokens(a));
+    const int all_see = job_seen(a, *job, first);
     float m = -INFINITY, l = 0.f;
+    // key tiles: t0, t0 + 1, ..., or every second one from t0 + t on
+    const int count = split ? (job->t1 - t0 + 1 - t) / 2 : job->end[t] - t0;
+    const int step = split ? 2 * kTileKeys : kTileKeys;
+    int base = (split ? t0 + t : t0) * kTileKeys;
 
-    for (int j = t0; j < end; ++j, ++done) {
+    for (int left = count; left > 0; --left, ++done, base += step) {
       if (ctrl->abort || !mbar_wait(&bars[C::kSFull + t], done & 1)) return false;
       if (idle) {
         mbar_arrive(&bars[C::kPFull + t]);
         continue;
       }
       tc_fence_after();
-      if (threadIdx.x == 0 && done == 0) FA_TRACE_CTA(2);
       uint32_t sr[4][32];
       tmem_ld32(tS + 0, sr[0]);
       tmem_ld32(tS + 32, sr[1]);
@@ -463,7 +515,6 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
         for (int c = 0; c < 128; ++c) s[c] *= a.scale_log2;
         sl = 1.f;
       }
-      const int base = j * kTileKeys;
       if (base + kTileKeys > all_see) {
         const int lim = seen - base;
 #pragma unroll
@@ -486,7 +537,7 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
       if (!(mt < INFINITY)) sum = NAN;
       l = m == -INFINITY && mt < INFINITY ? 0.f : fmaf(l, corr, sum);
       // P V of the tile before has completed: S was issued after it
-      if (j > t0 && __any_sync(0xffffffffu, rescale)) {
+      if (left < count && __any_sync(0xffffffffu, rescale)) {
 #pragma unroll
         for (int h = 0; h < D / 32; ++h) {
           uint32_t o[32];
@@ -505,7 +556,6 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
       mbar_arrive(&bars[C::kPFull + t]);
     }
 
-    if (threadIdx.x == 0) FA_TRACE_CTA(3);
     const bool whole = job->whole();
     const Division d = ctrl->division;
     // A split item's parts are joined by the last CTA to finish one. If all
@@ -514,10 +564,51 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
     const uint32_t mine = job->t1 - t0;
     uint32_t arrived = 0;
     if (!whole && row == 0) arrived = __ldcg(counter);
-    const bool any = end > t0;  // O_t holds something of this part
+    const bool any = count > 0;  // O_t holds something of this part
     if (any) {
       if (!mbar_wait(&bars[C::kODone + t], (done - 1) & 1)) return false;
       tc_fence_after();
+    }
+    if (split) {
+      // Group 1 leaves its (m, l); group 0 takes its O from tensor memory
+      // (the same lanes), joins both there and finishes the rows alone.
+      if (t == 1) {
+        mix[row] = make_float2(m, l);
+        tc_fence_before();
+        mbar_arrive(&bars[C::kMix]);
+        const bool ok = mbar_wait(&bars[C::kMixed], mixes & 1);
+        ++mixes;
+        if (!ok) return false;
+        continue;
+      }
+      if (!mbar_wait(&bars[C::kMix], mixes & 1)) return false;
+      ++mixes;
+      tc_fence_after();
+      const float2 other = mix[row];
+      const bool some = other.y != 0.f;  // else its O is nothing
+      const float top = some ? fmaxf(m, other.x) : m;
+      const float w0 = l != 0.f ? fast_exp2(m - top) : 0.f;
+      const float w1 = some ? fast_exp2(other.x - top) : 0.f;
+      if (!idle) {
+#pragma unroll
+        for (int h = 0; h < D / 32; ++h) {
+          uint32_t o[32], p[32];
+          tmem_ld32(tO + 32 * h, o);
+          tmem_ld32(tO + D + 32 * h, p);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const float x = l != 0.f ? __uint_as_float(o[c]) * w0 : 0.f;
+            o[c] = __float_as_uint(some ? fmaf(__uint_as_float(p[c]), w1, x) : x);
+          }
+          tmem_st32(tO + 32 * h, o);
+        }
+        tmem_wait_st();
+      }
+      l = some ? fmaf(other.y, w1, l * w0) : l;
+      m = top;
+      tc_fence_before();
+      mbar_arrive(&bars[C::kMixed]);
     }
     const size_t out_row = static_cast<size_t>(job->token + max(tok, 0)) * a.H +
                            job->h * group + row % group;
@@ -573,7 +664,6 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
       p[D * kRows + row] = m;
       p[(D + 1) * kRows + row] = l;
       __threadfence();
-      if (threadIdx.x == 0) FA_TRACE_CTA(4);
       if (!meet()) return false;
       if (row == 0) {
         const uint32_t had = atomicAdd(counter, mine);
@@ -583,7 +673,6 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
       if (!meet()) return false;
       last = ctrl->join[t] != 0;
     }
-    if (threadIdx.x == 0) FA_TRACE_CTA(5);
     if (!last) continue;
     if (row == 0) *counter = 0;
     if (idle) continue;
@@ -655,7 +744,6 @@ __device__ bool soften(const PagedArgs &a, uint64_t *bars, Ctrl *ctrl) {
       }
     }
     __syncwarp();
-    if (threadIdx.x == 0) FA_TRACE_CTA(6);
   }
 }
 
@@ -672,7 +760,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   PlanSmem *ps = reinterpret_cast<PlanSmem *>(smem + C::kMiscOff);
   Ctrl *ctrl = reinterpret_cast<Ctrl *>(smem + C::kCtrlOff);
   static_assert(sizeof(Ctrl) <= 512, "Ctrl has its place");
-  if (threadIdx.x == 0) FA_TRACE_CTA(0);
   if (smem_u32(smem) & 1023u) {
     if (threadIdx.x == 0) record_error(FA_ERR_SMEM_ALIGN);
     return;
@@ -694,6 +781,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&bars[C::kODone + t], 1);
         mbar_init(&bars[C::kJoin + t], 128);
       }
+      mbar_init(&bars[C::kMix], 128);
+      mbar_init(&bars[C::kMixed], 128);
       for (int p = 0; p < kParts; ++p) {
         mbar_init(&bars[C::kPartFull + p], 1);
         mbar_init(&bars[C::kPartEmpty + p], 11);  // warps that take parts
@@ -707,7 +796,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   });
   if (!work) return;
-  if (threadIdx.x == 0) FA_TRACE_CTA(1);
   if (threadIdx.x == 0) ctrl->division = d;
   if (warp == kMmaWarp) {
     tmem_alloc(&ctrl->tmem, 512);
@@ -731,7 +819,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     setmaxnreg_inc<kSoftmaxRegs>();
-    if (!soften<D, Dt>(a, bars, ctrl)) ctrl->abort = 1;
+    if (!soften<D, Dt>(a, bars, ctrl, reinterpret_cast<float2 *>(smem + C::kMixOff)))
+      ctrl->abort = 1;
   }
   tc_fence_before();
   __syncthreads();

@@ -380,3 +380,59 @@ def test_refusals():
     append_refuses("positions must be", freqs=freqs, positions=c.rows[:3])
     append_refuses("amplitude", freqs=freqs, amplitude=math.inf)
     clean()
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(page_rows=24, heads=8, kv_heads=8, dim=128, steps=6)])
+def test_server_loop_matches_whole_sequences(kw):
+    """paged_serving.py: chunks and single tokens through pages, against rope()
+    and prefill(). Both sides round the attention's output to bf16 and carry it
+    through two products: a relative difference of a few 2^-8 at most."""
+    import paged_serving
+
+    assert paged_serving.main(**kw) <= 4 * 2.0 ** -8
+
+
+def test_groups_that_share_the_keys_of_one_tile():
+    """At head_dim 64 an item of one query tile has its key tiles split between
+    two softmax groups: odd and even counts, rows that one group's tiles show
+    nothing, parts of long items."""
+    for news, lens in (([20], [129]), ([20], [385]), ([128], [128]), ([100, 3], [612, 1025]),
+                       ([40], [30]), ([17], [30000]), ([128, 128], [257, 20000])):
+        for dtype in (F16, BF16):
+            c = Paged(news, lens, 2, 2, 64, 64, dtype, seed=len(news) + news[0])
+            for causal in (True, False):
+                out, lse = attend(c, causal=causal, return_lse=True)
+                check_attention(c, out, 0.125, causal, lse)
+    # a wide group: one token is a tile's worth of rows
+    c = Paged([1, 1, 1], [700, 5000, 90], 40, 2, 64, 16, F16, seed=1)
+    check_attention(c, attend(c), 0.125)
+    clean()
+
+
+@pytest.mark.parametrize("h,h_kv", [(128, 1), (100, 1), (66, 2), (17, 1)])
+def test_wide_groups(h, h_kv):
+    for d, news, lens in ((64, [1, 3], [300, 77]), (128, [2, 1], [700, 33])):
+        c = Paged(news, lens, h, h_kv, d, 32, BF16, seed=h)
+        check_attention(c, attend(c), d ** -0.5)
+    clean()
+
+
+def test_special_values_in_the_cache():
+    """A NaN or an infinity of a row that a token sees reaches it; one past what
+    the sequence holds, or in another sequence, does not."""
+    for news in ([1, 1], [40, 3]):
+        for d in (64, 128):
+            c = Paged(news, [300, 200], 4, 2, d, 16, F16, seed=d)
+            clean_out = attend(c, causal=False)
+            c.kp[c.table[0, 7].long(), 0, 3, 5] = float("nan")
+            out = attend(c, causal=False)
+            n = news[0]
+            assert out[:n, :2].isnan().all()
+            assert torch.equal(out[:n, 2:], clean_out[:n, 2:])
+            assert torch.equal(out[n:], clean_out[n:])
+            c.kp[c.table[0, 7].long(), 0, 3, 5] = 0
+            c.vp[c.table[0, 7].long(), 1, 3, 5] = float("inf")
+            out = attend(c, causal=False)
+            assert (out[:n, 2:, 5] == float("inf")).all()
+            assert out[:n, :2].isfinite().all() and torch.equal(out[n:], clean_out[n:])
+    clean()
