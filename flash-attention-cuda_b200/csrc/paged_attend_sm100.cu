@@ -58,8 +58,12 @@ size_t attend_paged_workspace_bytes(int head_dim, int sms) {
   return 2 * static_cast<size_t>(sms) * many * sizeof(float);
 }
 
-// The few-row form reads the cache once for 16 query rows of a sequence and
-// head; the lengths are on the device, so the rule goes by their mean.
+// The few-row form reads the cache once for up to 16 query rows of a sequence
+// and head, the many-row form for up to 256. Measured with 32 sequences of
+// 4000 rows, 32 heads (us, few / many): 1 token, 16 rows of 128: 41.6 / 44.9;
+// 4 tokens x 4 heads of 128: 97 / 110; 5 x 4: 168 / 111; 4 x 4 of 64: 57 / 67;
+// 5 x 4 of 64: 93 / 67. The lengths are on the device, so the rule goes by the
+// mean; either form is right for every step.
 int attend_paged_form(const PagedArgs &a) {
   const long long group = a.H / a.H_kv;
   return group <= paged::few::kRows &&
@@ -68,6 +72,14 @@ int attend_paged_form(const PagedArgs &a) {
              : kPagedMany;
 }
 
+// The division of the work: what starting and finishing an item costs, in
+// keys; the least piece for which another CTA is taken on; the items that are
+// not worth a split. Swept on the shapes of the paged tests and 20 more; e.g.
+// item_cost 128 / 256 / 384: 64 ragged sequences of up to 8192 rows 177 / 163
+// / 161 us, 16 x 324 tokens over 5700 rows 240 / 203 / 192; items of up to 7
+// tiles split (few-row form): 64 sequences of up to 600 rows 17.3 us, whole
+// 10.1; pieces of 640 keys at least: 3000 rows of 2 heads 13.8 us, of 400
+// 13.0; many-row form, 768 / 512 / 384: 300 tokens, 8 K/V heads 32 / 30 / 17.5.
 void attend_paged_plan(PagedArgs &a, int form) {
   const int group = a.H / a.H_kv;
   a.box_rows = paged::box_rows(a.page_rows);

@@ -24,6 +24,12 @@
 //   9          MMA issuer (one elected thread); owns the TMEM allocation
 //   11         walks the CTA's parts and hands them to the others
 //
+// Measured (B200, device time): 2048 tokens over 16384 rows, 32 / 8 heads of
+// 128, 410-417 us (1240 TFLOP/s, 0.74 of cuBLAS; tensor pipe 62 % busy, MUFU
+// 39 %, a softmax warp waits for its tile most of the rest); the same with
+// heads of 64 340 us (760 TFLOP/s); 12 ragged sequences of up to 700 new tokens,
+// 12 heads of 64, 60 us.
+//
 // Shared memory: Q_t (128 rows x D), then a ring of key tiles (K and V, 128
 // rows x D each: 2 at D 128, 5 at 64), rows as 128-byte-swizzled halves of
 // 64 dims. Tensor memory: S_t at 128 t (P_t over its first 64 columns), O_t

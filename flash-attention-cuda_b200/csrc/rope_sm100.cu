@@ -11,10 +11,16 @@
 // latency for a generation step. A warp takes tokens, and of each some or all
 // rows (heads of q, k and v). A lane keeps to one unit of the rows, 16 bytes
 // (twice, in each half, where pairs are half a head apart), so its cosines and
-// sines stay in registers for all of a token's rows. A token's
-// first loads are issued before anything else; behind them the warp finds the
-// token's cache row and forms the cosines and sines, a pair or two a lane,
-// handed round through shared memory without a block-wide barrier.
+// sines stay in registers for all of a token's rows. A token's first loads are
+// issued before anything else; behind them the warp finds the token's cache row
+// and forms the cosines and sines, a pair or two a lane, handed round through
+// shared memory without a block-wide barrier.
+//
+// Measured (B200, device time): 2 x 40 x 5001 rows of 128, gradient, half of
+// the head rotated, 36.3 us (5.65 TB/s); prompt chunks of 6 sequences, 32 + 8 +
+// 8 heads of 128 into 16-row pages, 44 us (5.7 TB/s); 4 x 16 x 4096 rows of 64
+// 18.7 us (3.6 TB/s: at 16 rows of 128 bytes a token its instructions bound it,
+// 2.5 a cycle and SM of 4); one step of 64 sequences 4 us.
 
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -182,7 +188,7 @@ __global__ void __launch_bounds__(32 * kWarps) rope_kernel(const RopeArgs a) {
     double position = 0.;
     long long k_at = 0, v_at = 0;
     bool ready = false, skip = false;
-#pragma unroll 1
+#pragma unroll
     for (int sec = 0; sec < kSections; ++sec) {
       const int before = sec == 0 ? 0 : sec == 1 ? a.k_before : a.v_before;
       const int row1 = row_lane < a.row_lanes
@@ -312,6 +318,8 @@ cudaError_t launch(const RopeArgs &args, int sms, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
+// vector: rows in units of 16 bytes, where alignment and rotary_dim allow it;
+// element by element elsewhere.
 template <typename Dt, bool kAppend>
 cudaError_t pick(const RopeArgs &a, bool interleaved, bool vector, int sms,
                  cudaStream_t stream) {
