@@ -436,3 +436,23 @@ def test_special_values_in_the_cache():
             assert (out[:n, 2:, 5] == float("inf")).all()
             assert out[:n, :2].isfinite().all() and torch.equal(out[n:], clean_out[n:])
     clean()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n", [1, 40])
+def test_small_probabilities_keep_their_precision(dtype, n):
+    """One row far above all others, whose values are zero: the result is the
+    others' weights alone, about e^-13 each, below fp16's normal numbers."""
+    for d in (64, 128):
+        c = Paged([n], [500], 4, 2, d, 16, dtype)
+        c.q.zero_()[..., 0] = 1
+        for pages, rows in ((c.kp, c.k[0]), (c.vp, c.v[0])):
+            rows.zero_()
+            rows[1:, :, 0] = -13 if rows is c.k[0] else 1
+            pages.zero_()
+            for r0 in range(0, 500, 16):
+                m = min(16, 500 - r0)
+                pages[c.table[0, r0 // 16].long(), :, :m] = rows[r0:r0 + m].transpose(0, 1)
+        out = flashattn_cuda.attend_paged(c.q, c.starts, c.kp, c.vp, c.table, c.seq_lens, 1.0)
+        check_attention(c, out, 1.0)
+    clean()
