@@ -86,7 +86,9 @@ void attend_paged_plan(PagedArgs &a, int form) {
   a.min_part = 2;
   if (form == kPagedFew) {
     a.item_tokens = paged::few::kRows / group;
-    a.item_cost = 384;
+    // about 2.2 us at an SM's share of HBM; 384 / 512 keys at D 64: 64 ragged
+    // sequences 94 / 89 us, at D 128: 158 / 161
+    a.item_cost = a.D == 64 ? 512 : 384;
     a.min_piece = 400;
     a.whole_tiles = 7;
   } else {
