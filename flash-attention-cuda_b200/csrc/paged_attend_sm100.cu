@@ -24,13 +24,11 @@ cudaError_t launch(const PagedArgs &a, int form, const CUtensorMap &tm_q,
                    const CUtensorMap &tm_k, const CUtensorMap &tm_v, int sms,
                    cudaStream_t stream) {
   if (form == kPagedFew)
-    few::attend_few_kernel<D, Dt>
-        <<<min(sms, few::kMaxGrid), few::Cfg<D>::kThreads, few::Cfg<D>::kSmemBytes, stream>>>(a, tm_k, tm_v);
-  else
-    many::attend_many_kernel<D, Dt>
-        <<<sms, many::kThreads, many::Cfg<D>::kSmemBytes, stream>>>(a, tm_q, tm_k,
-                                                                   tm_v);
-  return cudaGetLastError();
+    return launch_early(few::attend_few_kernel<D, Dt>, dim3(min(sms, few::kMaxGrid)),
+                        few::Cfg<D>::kThreads, few::Cfg<D>::kSmemBytes, stream, a, tm_k,
+                        tm_v);
+  return launch_early(many::attend_many_kernel<D, Dt>, dim3(sms), many::kThreads,
+                      many::Cfg<D>::kSmemBytes, stream, a, tm_q, tm_k, tm_v);
 }
 
 }  // namespace paged

@@ -453,6 +453,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   uint64_t *copies = empty + C::kStages;
   PlanSmem *ps = reinterpret_cast<PlanSmem *>(smem + C::kMiscOff);
   if (smem_u32(smem) & 1023u) {
+    wait_for_stream();
     if (threadIdx.x == 0) record_error(FA_ERR_SMEM_ALIGN);
     return;
   }

@@ -770,6 +770,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Ctrl *ctrl = reinterpret_cast<Ctrl *>(smem + C::kCtrlOff);
   static_assert(sizeof(Ctrl) <= 512, "Ctrl has its place");
   if (smem_u32(smem) & 1023u) {
+    wait_for_stream();
     if (threadIdx.x == 0) record_error(FA_ERR_SMEM_ALIGN);
     return;
   }

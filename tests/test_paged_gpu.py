@@ -456,3 +456,43 @@ def test_small_probabilities_keep_their_precision(dtype, n):
         out = flashattn_cuda.attend_paged(c.q, c.starts, c.kp, c.vp, c.table, c.seq_lens, 1.0)
         check_attention(c, out, 1.0)
     clean()
+
+
+@pytest.mark.parametrize("n", [1, 50])
+def test_calls_in_a_row_wait_for_one_another(n):
+    """A chain in which every call reads what the one before it wrote (rows
+    appended, queries made from the last output): the same bits with and
+    without a synchronisation after each."""
+    h, h_kv, d, steps, b = 8, 2, 64, 40, 3
+    freqs, _ = flashattn_cuda.rope_frequencies(d)
+    torch.manual_seed(n)
+    first = torch.randn(b * n, h + 2 * h_kv, d, device="cuda").half()
+    starts = torch.arange(0, b * n + 1, n, device="cuda", dtype=torch.int32)
+    pages = steps * n // 16 + 1
+    table = torch.randperm(b * pages, device="cuda", dtype=torch.int32).view(b, pages)
+
+    def chain(wait):
+        kp = torch.zeros(b * pages, h_kv, 16, d, device="cuda").half()
+        vp = torch.zeros_like(kp)
+        x, outs = first, []
+        lens = torch.zeros(b, device="cuda", dtype=torch.int32)
+        for _ in range(steps):
+            lens += n
+            q = flashattn_cuda.append_paged(x[:, h:h + h_kv], x[:, h + h_kv:], starts, kp, vp,
+                                            table, lens, q=x[:, :h], freqs=freqs)
+            wait()
+            o = flashattn_cuda.attend_paged(q, starts, kp, vp, table, lens, 0.125)
+            wait()
+            o = flashattn_cuda.attend_paged(o * 4, starts, kp, vp, table, lens, 0.125)
+            wait()
+            x = (x * 0.5 + torch.cat((o, o[:, :2 * h_kv]), 1)).clamp(-3, 3)  # stays finite
+            outs.append(o)
+        torch.cuda.synchronize()
+        return torch.stack(outs), kp, vp
+
+    want = chain(torch.cuda.synchronize)
+    assert want[0].isfinite().all()
+    for _ in range(3):
+        for a, c in zip(chain(lambda: None), want):
+            assert torch.equal(a, c)
+    clean()
