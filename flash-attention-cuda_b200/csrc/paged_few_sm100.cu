@@ -16,10 +16,10 @@
 // second product rounded to the tensors' 16-bit type, as the MMA takes it.
 //
 // Measured (B200, device time): 64 ragged sequences of up to 8192 rows, 32 / 8
-// heads of 128, 159 us (6.3 TB/s, 0.98 of the copy bandwidth); one sequence of
-// 131072 rows, 14 / 2 heads of 64, 24.8 us (10.4 at that bandwidth: the rest is
-// 4 us until the first tile, 1.3 to join the warps, 6 to join 74 parts); one
-// sequence of 701 rows 9.8 us.
+// heads of 128, 156 us (6.45 TB/s, the copy bandwidth); one sequence of 131072
+// rows, 14 / 2 heads of 64, 24.6 us (10.4 at that bandwidth: the rest is 4 us
+// until the first tile, 1.3 to join the warps, 6 to join 74 parts); one sequence
+// of 701 rows 9.5 us.
 
 #include <cuda.h>
 #include <cuda_fp16.h>

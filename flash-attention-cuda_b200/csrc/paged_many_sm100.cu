@@ -25,7 +25,7 @@
 //   11         walks the CTA's parts and hands them to the others
 //
 // Measured (B200, device time): 2048 tokens over 16384 rows, 32 / 8 heads of
-// 128, 410-417 us (1240 TFLOP/s, 0.74 of cuBLAS; tensor pipe 62 % busy, MUFU
+// 128, 407-417 us (1250 TFLOP/s, 0.75 of cuBLAS; tensor pipe 62 % busy, MUFU
 // 39 %, a softmax warp waits for its tile most of the rest); the same with
 // heads of 64 340 us (760 TFLOP/s); 12 ragged sequences of up to 700 new tokens,
 // 12 heads of 64, 60 us.

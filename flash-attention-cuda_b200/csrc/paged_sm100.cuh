@@ -22,31 +22,6 @@
 
 namespace fa {
 
-// A kernel launched with launch_early() may start while the one before it in
-// the stream still runs: nothing of global memory is read or written before
-// this (every thread of the grid comes through it). Back to back calls on one
-// sequence of 701 rows took 13.6 us without, 9.2 so.
-__device__ __forceinline__ void wait_for_stream() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
-// Launches a kernel whose start overlaps the end of the one before it.
-template <typename... P, typename... A>
-cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t smem,
-                         cudaStream_t stream, const A &...args) {
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 namespace paged {
 
 // 4-D tiled TMA load; coordinates are innermost first.

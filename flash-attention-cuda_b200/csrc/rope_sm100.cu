@@ -17,10 +17,10 @@
 // shared memory without a block-wide barrier.
 //
 // Measured (B200, device time): 2 x 40 x 5001 rows of 128, gradient, half of
-// the head rotated, 36.3 us (5.65 TB/s); prompt chunks of 6 sequences, 32 + 8 +
+// the head rotated, 36.1 us (5.7 TB/s); prompt chunks of 6 sequences, 32 + 8 +
 // 8 heads of 128 into 16-row pages, 44 us (5.7 TB/s); 4 x 16 x 4096 rows of 64
-// 18.7 us (3.6 TB/s: at 16 rows of 128 bytes a token its instructions bound it,
-// 2.5 a cycle and SM of 4); one step of 64 sequences 4 us.
+// 18.8 us (3.6 TB/s: at 16 rows of 128 bytes a token its instructions bound it,
+// 2.5 a cycle and SM of 4); one step of 64 sequences 3.3 us.
 
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(32 * kWarps) rope_kernel(const RopeArgs a) {
   __shared__ float2 turns_of[kWarps][kMaxPairs];  // (cos, sin) * amplitude
   float2 *turns = turns_of[threadIdx.x >> 5];
   const int lane = threadIdx.x & 31;
+  wait_for_stream();
   const uint32_t w = blockIdx.x * kWarps + (threadIdx.x >> 5);
   const int first_token = static_cast<int>(w / static_cast<uint32_t>(a.chunks));
   const int chunk = static_cast<int>(w) - first_token * a.chunks;
@@ -314,8 +315,8 @@ cudaError_t launch(const RopeArgs &args, int sms, cudaStream_t stream) {
   a.token_step = static_cast<int>(want > a.tokens ? a.tokens : want < 1 ? 1 : want);
   const long long warps = static_cast<long long>(a.token_step) * a.chunks;
   const unsigned grid = static_cast<unsigned>((warps + kWarps - 1) / kWarps);
-  rope_kernel<Dt, V, kInterleaved, kAppend><<<grid, 32 * kWarps, 0, stream>>>(a);
-  return cudaGetLastError();
+  return launch_early(rope_kernel<Dt, V, kInterleaved, kAppend>, dim3(grid), 32 * kWarps, 0,
+                      stream, a);
 }
 
 // vector: rows in units of 16 bytes, where alignment and rotary_dim allow it;
